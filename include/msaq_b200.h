@@ -350,6 +350,78 @@ int msaq_kv_decode_attention_rope(const void* q,
                                   int64_t q_pos, const int32_t* q_pos_per_seq,
                                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------- a step with several drafted tokens -- */
+
+/*
+ * One speculative decoding step (no reference counterpart: the reference decodes one token per sequence and step).  T drafted tokens per
+ * sequence, node 0 the root -- the last token chosen, which the cache does not hold yet --, the others hanging on it as a tree
+ * (a chain, one token, are trees), go through the model together:
+ *   msaq_kv_write_qkv       per layer: the nodes' queries out, their keys and values into slots len + i
+ *   msaq_kv_tree_attention  per layer: every node attends the len keys in front and its own ancestors
+ *   msaq_verify_tree        once: which nodes stay, and the token behind them
+ *   msaq_kv_keep            per layer: the rows of the nodes that stay move to slots len, len + 1, ...
+ * All four read lengths, positions, masks and decisions from device memory and can be captured.
+ *
+ * msaq_kv_write_qkv.  qkv bf16: B*T tokens, `ld` elements from one to the next, each [H + 2 Hkv][D] (queries, keys, values).  A query
+ * row becomes q_out [B][T][H][D] = bf16(rope(norm(x))), a key row bf16(rope(norm(x))), Hadamard-rotated when rotate_k != 0 and
+ * quantised, a value row is quantised: the bytes of msaq_kv_append_pair on the bf16 rows.  norm(x) = (x r) g with r =
+ * fl32((mean(x^2) + eps)^(-1/2)), mean and root in 64 bits; q_gain / k_gain [D] bf16 or fp32 (gain_is_f32), NULL: no norm.
+ * Token t of sequence b goes to slot (start_per_seq ? start_per_seq[b] : start) + t; its position is pos[b*T + t] when pos is
+ * given, else the slot.  RoPE tables as for msaq_rope, rows indexed by position (rope_rows == 1, one position, only with T == 1);
+ * rope_cos == NULL: no RoPE.  counts[b] when given: only the first counts[b] tokens of a sequence are there; the
+ * query rows of the others are 0 and nothing is written for them.  A slot outside [0, Lcap) or a position outside the tables that
+ * comes from device memory sets MSAQ_STATUS_BAD_APPEND_POS: the key and value rows are skipped (a query row is rotated by the
+ * nearest position of the tables).  T is any length: a prompt goes through the same call.
+ */
+int msaq_kv_write_qkv(const void* qkv, int64_t ld, void* q_out, int8_t* k_scale_exp, uint8_t* k_upper, uint8_t* k_shared,
+                      int8_t* v_scale_exp, uint8_t* v_upper, uint8_t* v_shared, int64_t B, int64_t T, int64_t H, int64_t Hkv,
+                      int64_t D, int64_t NB, int64_t start, const int32_t* start_per_seq, const int32_t* pos,
+                      const int32_t* counts, const void* q_gain, const void* k_gain, int gain_is_f32, double eps,
+                      const float* rope_cos, const float* rope_sin, int64_t rope_rows, int64_t Lcap, int u, int gs,
+                      int rotate_k, void* stream);
+
+/*
+ * q, out [B][T][H][D] bf16, T <= 64; node i of sequence b attends the keys [0, len_b) and, for every bit j of its mask word, slot
+ * len_b + j; a node that attends nothing gives 0.  mask: uint64 [B][T] (mask_stride elements from one sequence to the next) or one
+ * tree [T] for all (mask_stride 0).  Bits at or beyond T count for nothing, and neither do slots that no bit names, whatever
+ * they hold.  lens int32 [B], clipped to [0, Lk - T]; NULL: Lk - T for every sequence.  Lk: keys that any sequence can attend, the
+ * nodes included (it sets the split of the keys).  qrot as for msaq_kv_decode_attention_batched.  Any H / Hkv; formats and head
+ * dimensions as for the decode.  out_f32 (optional) also receives the result before its rounding.
+ */
+size_t msaq_kv_tree_workspace(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk, int64_t D);
+int msaq_kv_tree_attention(const void* q, const int8_t* ks, const uint8_t* ku, const uint8_t* kh,
+                           const int8_t* vs, const uint8_t* vu, const uint8_t* vh, void* out, float* out_f32,
+                           const int32_t* lens, const uint64_t* mask, int64_t mask_stride,
+                           int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk, int64_t D, int64_t NB, int u, int gs,
+                           int64_t Lcap, int qrot, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Recursive rejection sampling down the tree.  target_probs [B][T][V] (strides in elements, the last one 1; fp32 or bf16, draft_probs
+ * the same): row i is the target's distribution behind node i.  draft_probs: row i is the distribution that the children
+ * of node i were drawn from, each by itself; NULL: the children were chosen, not drawn.  tokens, uniforms [B][T]: a node's
+ * token and its random number in [0, 1) (entry 0: the final draw's).  parents [B][T] or [T] (parents_stride_b 0): -1 for the root
+ * and for nodes that are not there; a node whose parent is not in front of it, or whose token is outside [0, V), is not there
+ * either.  From the root, cur, r = p_cur, Z = 1: children of cur in index order; child j with token x is accepted if
+ *   u_j q(x) Z < r(x)       (q(x) = 1 without draft_probs)
+ * -- then cur = j and it begins anew -- and rejected otherwise: r = max(r - Z q, 0), Z = sum(r) (without draft_probs r(x) = 0,
+ * Z -= r(x)).  Where no child is left: token[b] = the first t with r(0) + ... + r(t) > u_0 sum(r); p_cur takes r's place where
+ * nothing is left of it, and token[b] = -1 where p_cur has nothing either.  Entries that are not positive and finite count as 0;
+ * sums are in 64 bits.  path[b] = the accepted nodes, the root first, then -1; count[b] = how many, the root included.
+ */
+int msaq_verify_tree(const void* target_probs, int64_t target_stride_b, int64_t target_stride_t, const void* draft_probs,
+                     int64_t draft_stride_b, int64_t draft_stride_t, int probs_are_f32, const int32_t* tokens,
+                     const int32_t* parents, int64_t parents_stride_b, const float* uniforms, int32_t* path, int32_t* count,
+                     int32_t* token, int64_t B, int64_t T, int64_t V, void* stream);
+
+/*
+ * In both caches slot start + k takes what slot start + path[b][k] held before the call, k < count[b] (path, count as msaq_verify_tree
+ * writes them, start as for msaq_kv_write_qkv, T <= 64); all other slots stay.  A node outside [0, T) or a slot outside [0, Lcap)
+ * sets MSAQ_STATUS_BAD_APPEND_POS and that row is skipped.
+ */
+int msaq_kv_keep(int8_t* k_scale_exp, uint8_t* k_upper, uint8_t* k_shared, int8_t* v_scale_exp, uint8_t* v_upper,
+                 uint8_t* v_shared, const int32_t* path, const int32_t* count, int64_t start, const int32_t* start_per_seq,
+                 int64_t B, int64_t T, int64_t Hkv, int64_t NB, int64_t Lcap, int u, int gs, void* stream);
+
 /* ------------------------------------------------- tensor-parallel exchange -- */
 
 /*

@@ -68,6 +68,13 @@ SIGNATURES = {
     "msaq_mxint8_kv_write": (_int, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "msaq_mxint8_kv_decode_batched": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                              _p, _sz, _p]),
+    "msaq_kv_write_qkv": (_int, [_p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p,
+                                 _int, C.c_double, _p, _p, _i64, _i64, _int, _int, _int, _p]),
+    "msaq_kv_tree_workspace": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "msaq_kv_tree_attention": (_int, [_p] * 7 + [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _i64,
+                                                 _int, _p, _sz, _p]),
+    "msaq_verify_tree": (_int, [_p, _i64, _i64, _p, _i64, _i64, _int, _p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p]),
+    "msaq_kv_keep": (_int, [_p] * 8 + [_i64, _p, _i64, _i64, _i64, _i64, _i64, _int, _int, _p]),
     "msaq_rmsnorm": (_int, [_p, _p, _i64, _i64, C.c_float, _p]),
     "msaq_silu_mul": (_int, [_p, _p, _i64, _i64, _p]),
     "msaq_add_residual": (_int, [_p, _p, _int, _p, _i64, _p]),

@@ -8,19 +8,13 @@
 // Behaviour replaced: csrc/kv_attention.cu:450-829 and :1220-1244.
 #pragma once
 
-#include "msaq_common.cuh"
+#include "kv_planes.cuh"
 #include "sm100_ptx.cuh"
 
 namespace msaq {
 
 constexpr int KVG_THREADS = 128;
 constexpr int KVG_CHUNK = 128;
-
-struct KvPlanes {
-    const int8_t* s;
-    const uint8_t* u;
-    const uint8_t* h;
-};
 
 // Partial layout per (b, head, tile): D floats of acc, then m, then l.
 __host__ __device__ inline int64_t kv_partial_stride(int D) { return D + 2; }
@@ -47,21 +41,6 @@ __device__ __forceinline__ float kv_block_dot(const uint8_t* up_bytes, const uin
         dot = fmaf((float)(up * (1 << U) + sh), qv[k], dot);
     }
     return dot;
-}
-
-// One dequantised element (block-local index k) of the record at `slot`.
-__device__ __forceinline__ float kv_element(const KvPlanes& p, int64_t slot, int k, const Fmt& f) {
-    const uint8_t* ub = p.u + slot * f.UB;
-    const int bit = k * f.wbits, by = bit >> 3, off = bit & 7;
-    uint32_t v = ub[by] >> off;
-    if (off + f.wbits > 8) v |= (uint32_t)ub[by + 1] << (8 - off);
-    const int up = sext(v, f.wbits);
-    const uint8_t* sb = p.h + slot * f.SB;
-    const int sbit = (k >> f.lg_gs) * f.u, sby = sbit >> 3, soff = sbit & 7;
-    uint32_t w = sb[sby] >> soff;
-    if (soff + f.u > 8) w |= (uint32_t)sb[sby + 1] << (8 - soff);
-    const int sh = sext(w, f.u);
-    return (float)(up * (1 << f.u) + sh) * exp2_int((int)p.s[slot]);
 }
 
 template <int U>

@@ -1,0 +1,381 @@
+// From the QKV projection's output to attention in one launch: norms of the query and key heads, rotary embedding, the query
+// rows out in bf16, the key rows (Hadamard-rotated where the cache is) and the value rows quantised into the cache -- for one
+// token, for the nodes of a drafted tree (whose positions differ from their slots) and for a prompt.  And the move that follows
+// the verification of a drafted tree: the accepted nodes' rows become neighbours.
+//
+// A head row x with gain g becomes  y = bf16( rope( (x r) g ) ),  r = fl32( (mean(x^2) + eps)^(-1/2) ).  Mean and root are taken
+// in 64 bits: r is then the same number however the sum is split over lanes, and so are the codes that the quantiser derives from
+// y (in 32 bits one key row in about ten thousand would land on other codes).  The remaining steps are fp32 operations,
+// each rounded by itself.
+//
+// What bounds it: a token moves 2 D (2 Hq + 2 Hkv) + 2 Hkv NB (UB + SB + 1) bytes, so HBM for a prompt and launch and
+// latency for one token.
+#include "kv_quant_row.cuh"
+
+namespace msaq {
+namespace {
+
+constexpr int QKV_WARPS = 4;
+constexpr int KEEP_MAX_T = 64;
+
+struct QkvArgs {
+    const __nv_bfloat16* x;              // [B * T] tokens of Hq + 2 Hkv heads, ld elements from one token to the next
+    __nv_bfloat16* q_out;                // [B * T][Hq][D]
+    QuantJob k, v;
+    int64_t ld, start, Lcap;
+    const int32_t* start_per_seq;
+    const int32_t* pos;                  // optional [B][T]: positions; null: the slots
+    const int32_t* counts;               // optional [B]: tokens of a sequence, the rest is padding
+    const void* q_gain;                  // optional [D]
+    const void* k_gain;
+    Rope rope;
+    double eps;
+    int* sticky;
+    int B, T, Hq, Hkv, gain_f32;
+    bool wide;                           // x, ld and q_out allow 16-byte accesses
+    int64_t q_blocks, k_blocks;          // thread blocks of the query rows, of the key rows (as many of the value rows)
+};
+
+// (mean + eps)^(-1/2) rounded to fp32: one Newton step of third order in 64 bits on the 32-bit estimate (relative error
+// below 2^-60); a sum beyond the range of fp32 takes the slow root.
+__device__ __forceinline__ float norm_factor(double ss, int D, double eps) {
+    const double m = ss / (double)D + eps;
+    if (!(m > 1e-36 && m < 1e36)) return (float)(1.0 / sqrt(m));
+    const double y = (double)rsqrtf((float)m);
+    const double e = fma(-m * y, y, 1.0);
+    return (float)fma(y * e, fma(0.375, e, 0.5), y);
+}
+
+__device__ __forceinline__ float gain_at(const void* g, int f32, int i) {
+    return f32 ? static_cast<const float*>(g)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i]);
+}
+
+// Where a row goes: its token's sequence, slot and position.  `live` on return: not padding (q), and its slot inside the cache (k, v).
+struct QkvRow {
+    int64_t token, key, at;
+    int head, b;
+    bool live;
+};
+
+__device__ __forceinline__ QkvRow qkv_row(const QkvArgs& a, int64_t row, int heads, bool into_cache, bool report) {
+    QkvRow r;
+    const int64_t rows = (int64_t)a.B * a.T * heads;
+    r.live = row < rows;
+    if (!r.live) row = 0;
+    if (rows <= UINT32_MAX) {
+        const uint32_t tok = (uint32_t)row / (uint32_t)heads;
+        r.head = (int)((uint32_t)row - tok * (uint32_t)heads);
+        r.b = (int)(tok / (uint32_t)a.T);
+        r.token = tok;
+    } else {
+        r.token = row / heads;
+        r.head = (int)(row % heads);
+        r.b = (int)(r.token / a.T);
+    }
+    const int t = (int)(r.token - (int64_t)r.b * a.T);
+    if (a.counts && t >= a.counts[r.b]) r.live = false;
+    r.key = (a.start_per_seq ? (int64_t)a.start_per_seq[r.b] : a.start) + t;
+    r.at = a.pos ? (int64_t)a.pos[r.token] : r.key;
+    bool bad = into_cache && (r.key < 0 || r.key >= a.Lcap);
+    if (a.rope.cos) {
+        if (a.rope.rows == 1) r.at = 0;
+        const int64_t p = min(max(r.at, (int64_t)0), a.rope.rows - 1);
+        bad = bad || p != r.at;
+        r.at = p;
+    }
+    if (bad && r.live) {                                       // a position from device memory: the row is skipped, the status word says so
+        if (report && a.sticky) atomicOr(a.sticky, BAD_APPEND_POS);
+        if (into_cache) r.live = false;
+    }
+    return r;
+}
+
+// The gs = 2 formats: eight values per lane, 8 / EPL rows per warp, nothing through shared memory.
+template <int EPL, int U>
+__global__ void __launch_bounds__(QKV_WARPS * 32)
+qkv_write8_kernel(const QkvArgs a) {
+    chain_release();
+    chain_wait();
+    constexpr int D = 32 * EPL, LANES = 4 * EPL, ROWS = 8 / EPL;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES;
+    int64_t blk = blockIdx.x;
+    const int kind = blk < a.q_blocks ? 0 : blk < a.q_blocks + a.k_blocks ? 1 : 2;
+    blk -= kind == 0 ? 0 : kind == 1 ? a.q_blocks : a.q_blocks + a.k_blocks;
+    const int heads = kind == 0 ? a.Hq : a.Hkv, head0 = kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv;
+    const int64_t row = (blk * QKV_WARPS + warp) * ROWS + lane / LANES;
+    const QkvRow r = qkv_row(a, row, heads, kind != 0, l == 0);
+    const bool in_range = row < (int64_t)a.B * a.T * heads;
+    float v[8];
+    const __nv_bfloat16* src = a.x + r.token * a.ld + (int64_t)(head0 + r.head) * D + l * 8;
+    if (!r.live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    } else if (a.wide) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(src);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(w[i]); v[2 * i + 1] = bf16_hi(w[i]); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(src[i]);
+    }
+    if (kind != 2) {
+        const void* gain = kind == 0 ? a.q_gain : a.k_gain;
+        if (gain) {
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fma((double)v[i], (double)v[i], ss);
+#pragma unroll
+            for (int m = 1; m < LANES; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            const float f = norm_factor(ss, D, a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], f), gain_at(gain, a.gain_f32, l * 8 + i));
+        }
+        if (a.rope.cos) {
+            const int64_t at = r.at * (D / 2) + l * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                rope_pair(v[2 * i], v[2 * i + 1], a.rope.cos[at + i], a.rope.sin[at + i], &v[2 * i], &v[2 * i + 1]);
+        } else if (gain) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(__float2bfloat16_rn(v[i]));
+        }
+    }
+    if (kind == 0) {
+        if (!in_range) return;
+        __nv_bfloat16* dst = a.q_out + row * D + l * 8;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(r.live ? v[2 * i] : 0.0f, r.live ? v[2 * i + 1] : 0.0f);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (a.wide) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                dst[2 * i] = __ushort_as_bfloat16((unsigned short)(w[i] & 0xFFFFu));
+                dst[2 * i + 1] = __ushort_as_bfloat16((unsigned short)(w[i] >> 16));
+            }
+        return;
+    }
+    quantize_values8_warp<EPL, U>(v, kind == 1 ? a.k : a.v, (int64_t)r.b * a.Hkv + r.head, r.key, a.Lcap, r.live, lane);
+}
+
+// Every other group size: one warp per row, the lane-per-element quantiser.
+template <int EPL>
+__global__ void __launch_bounds__(QKV_WARPS * 32)
+qkv_write_kernel(const QkvArgs a, Fmt f) {
+    chain_release();
+    chain_wait();
+    constexpr int D = 32 * EPL, NB = EPL;
+    __shared__ float rowbuf[QKV_WARPS][D];
+    __shared__ uint32_t codes[QKV_WARPS][NB * QROW_CW];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int64_t blk = blockIdx.x;
+    const int kind = blk < a.q_blocks ? 0 : blk < a.q_blocks + a.k_blocks ? 1 : 2;
+    blk -= kind == 0 ? 0 : kind == 1 ? a.q_blocks : a.q_blocks + a.k_blocks;
+    const int heads = kind == 0 ? a.Hq : a.Hkv, head0 = kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv;
+    const int64_t row = blk * QKV_WARPS + warp;
+    if (row >= (int64_t)a.B * a.T * heads) return;             // whole warps
+    const QkvRow r = qkv_row(a, row, heads, kind != 0, lane == 0);
+    if (!r.live) {
+        if (kind == 0)
+            for (int i = lane; i < D; i += 32) a.q_out[row * D + i] = __float2bfloat16_rn(0.0f);
+        return;
+    }
+    float v[EPL];
+    const __nv_bfloat16* src = a.x + r.token * a.ld + (int64_t)(head0 + r.head) * D + lane * EPL;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) v[i] = __bfloat162float(src[i]);
+    if (kind != 2) {
+        const void* gain = kind == 0 ? a.q_gain : a.k_gain;
+        if (gain) {
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) ss = fma((double)v[i], (double)v[i], ss);
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            const float s = norm_factor(ss, D, a.eps);
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], s), gain_at(gain, a.gain_f32, lane * EPL + i));
+        }
+        if (a.rope.cos) rope_warp<EPL>(v, lane, a.rope, r.at);
+        else if (gain)
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) v[i] = __bfloat162float(__float2bfloat16_rn(v[i]));
+    }
+    if (kind == 0) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) a.q_out[row * D + lane * EPL + i] = __float2bfloat16_rn(v[i]);
+        return;
+    }
+    quantize_values_warp<EPL>(v, kind == 1 ? a.k : a.v, (int64_t)r.b * a.Hkv + r.head, r.key, a.Lcap, f, rowbuf[warp], codes[warp], lane);
+}
+
+template <int EPL>
+int launch_qkv(QkvArgs& a, const Fmt& f, bool rows8, cudaStream_t st) {
+    const int64_t per_block = (int64_t)QKV_WARPS * (rows8 ? 8 / EPL : 1), tokens = (int64_t)a.B * a.T;
+    a.q_blocks = (tokens * a.Hq + per_block - 1) / per_block;
+    a.k_blocks = (tokens * a.Hkv + per_block - 1) / per_block;
+    const int64_t blocks = a.q_blocks + 2 * a.k_blocks;
+    if (blocks > INT32_MAX) return fail(MSAQ_ERR_ARG, "size exceeds the supported range");
+    const dim3 grid((unsigned)blocks), block(QKV_WARPS * 32);
+    if (!rows8) launch_chained(qkv_write_kernel<EPL>, grid, block, 0, st, a, f);
+    else if (f.u == 4) launch_chained(qkv_write8_kernel<EPL, 4>, grid, block, 0, st, a);
+    else if (f.u == 3) launch_chained(qkv_write8_kernel<EPL, 3>, grid, block, 0, st, a);
+    else launch_chained(qkv_write8_kernel<EPL, 2>, grid, block, 0, st, a);
+    count_launch();
+    return check_launch("kv_write_qkv");
+}
+
+// ---- the accepted nodes' rows move together -------------------------------------------------------------
+struct KeepArgs {
+    int8_t* s[2];
+    uint8_t* up[2];
+    uint8_t* sh[2];
+    const int32_t* path;                 // [B][T]
+    const int32_t* count;                // [B]
+    const int32_t* start_per_seq;
+    int64_t start, Lcap;
+    int* sticky;
+    int T, Hkv, NB, UB, SB;
+    int64_t planes;                      // B * Hkv * NB
+};
+
+// One warp per (sequence, head, block) of one cache reads every row that moves into registers before it writes one, so a row
+// may go where another one comes from.  Two rows per lane cover the 64 nodes of the largest tree.
+__global__ void __launch_bounds__(128)
+keep_kernel(const KeepArgs a) {
+    chain_release();
+    chain_wait();
+    const int lane = threadIdx.x & 31, c = blockIdx.y;
+    const int64_t plane = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (plane >= a.planes) return;
+    const int b = (int)(plane / (a.Hkv * a.NB));
+    const int64_t start = a.start_per_seq ? (int64_t)a.start_per_seq[b] : a.start;
+    const int n = min(max(a.count[b], 0), a.T);
+    uint32_t up[2][6];
+    uint64_t sh[2];
+    int8_t e[2];
+    bool move[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int k = lane + 32 * i;
+        const int node = k < n ? a.path[(int64_t)b * a.T + k] : k;
+        const bool ok = node >= 0 && node < a.T && start >= 0 && start + max(node, k) < a.Lcap;
+        if (k < n && !ok && a.sticky) atomicOr(a.sticky, BAD_APPEND_POS);
+        move[i] = k < n && ok && node != k;
+        if (!move[i]) continue;
+        const int64_t from = plane * a.Lcap + start + node;
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(a.up[c] + from * a.UB);
+#pragma unroll
+        for (int w = 0; w < 6; ++w) up[i][w] = w * 4 < a.UB ? u[w] : 0u;
+        const uint8_t* h = a.sh[c] + from * a.SB;
+        sh[i] = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sh[i] |= w < a.SB ? (uint64_t)h[w] << (8 * w) : 0ull;
+        e[i] = a.s[c][from];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (!move[i]) continue;
+        const int64_t to = plane * a.Lcap + start + lane + 32 * i;
+        uint32_t* u = reinterpret_cast<uint32_t*>(a.up[c] + to * a.UB);
+#pragma unroll
+        for (int w = 0; w < 6; ++w)
+            if (w * 4 < a.UB) u[w] = up[i][w];
+        uint8_t* h = a.sh[c] + to * a.SB;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            if (w < a.SB) h[w] = (uint8_t)(sh[i] >> (8 * w));
+        a.s[c][to] = e[i];
+    }
+}
+
+}  // namespace
+}  // namespace msaq
+
+using namespace msaq;
+
+extern "C" int msaq_kv_write_qkv(const void* qkv, int64_t ld, void* q_out, int8_t* k_scale_exp, uint8_t* k_upper, uint8_t* k_shared,
+                                 int8_t* v_scale_exp, uint8_t* v_upper, uint8_t* v_shared, int64_t B, int64_t T, int64_t H,
+                                 int64_t Hkv, int64_t D, int64_t NB, int64_t start, const int32_t* start_per_seq, const int32_t* pos,
+                                 const int32_t* counts, const void* q_gain, const void* k_gain, int gain_is_f32, double eps,
+                                 const float* rope_cos, const float* rope_sin, int64_t rope_rows, int64_t Lcap, int u, int gs,
+                                 int rotate_k, void* stream) {
+    const DeviceScope device;
+    Fmt f;
+    if (!qkv || !q_out || !k_scale_exp || !k_upper || !k_shared || !v_scale_exp || !v_upper || !v_shared)
+        return fail(MSAQ_ERR_ARG, "null pointer");
+    if (!make_fmt(u, gs, &f)) return fail(MSAQ_ERR_UNSUPPORTED, "unsupported format u=%d gs=%d", u, gs);
+    if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || Lcap <= 0) return fail(MSAQ_ERR_ARG, "B, T, H, Hkv and Lcap must be positive");
+    if (B > INT32_MAX || T > INT32_MAX || H > 65535 || Hkv > 65535 || B * T > INT32_MAX)
+        return fail(MSAQ_ERR_ARG, "size exceeds the supported range");
+    if (D != 32 && D != 64 && D != 128 && D != 256)
+        return fail(MSAQ_ERR_UNSUPPORTED, "head_dim %lld: must be 32, 64, 128 or 256", (long long)D);
+    if (NB * BLOCK != D) return fail(MSAQ_ERR_ARG, "NB (%lld) must equal D/32 (D=%lld)", (long long)NB, (long long)D);
+    if (ld < (H + 2 * Hkv) * D) return fail(MSAQ_ERR_ARG, "ld (%lld) is smaller than a token's heads", (long long)ld);
+    if (!(eps >= 0.0)) return fail(MSAQ_ERR_ARG, "eps must not be negative");
+    if (!start_per_seq && (start < 0 || start + T > Lcap))
+        return fail(MSAQ_ERR_ARG, "slots [%lld, %lld) exceed the cache capacity %lld", (long long)start, (long long)(start + T), (long long)Lcap);
+    if ((rope_cos == nullptr) != (rope_sin == nullptr)) return fail(MSAQ_ERR_ARG, "rope_cos and rope_sin come together");
+    if (rope_cos) {
+        // a row per position: every slot that a token can go to needs its table row (given positions are checked on the device)
+        const int64_t need = pos ? 1 : start_per_seq ? Lcap : start + T;
+        if (rope_rows < 1 || (rope_rows == 1 && T > 1) || (rope_rows > 1 && rope_rows < need))
+            return fail(MSAQ_ERR_ARG, "the RoPE tables have %lld rows, %lld tokens with positions up to %lld are possible",
+                        (long long)rope_rows, (long long)T, (long long)need - 1);
+    }
+    if ((reinterpret_cast<uintptr_t>(k_upper) | reinterpret_cast<uintptr_t>(v_upper)) & 3)
+        return fail(MSAQ_ERR_ARG, "upper planes must be 4-byte aligned");
+    if (gain_is_f32 && ((reinterpret_cast<uintptr_t>(q_gain) | reinterpret_cast<uintptr_t>(k_gain)) & 3))
+        return fail(MSAQ_ERR_ARG, "gains must be aligned to their type");
+    if (int rc = require_sm100()) return rc;
+    QkvArgs a{};
+    a.x = static_cast<const __nv_bfloat16*>(qkv);
+    a.q_out = static_cast<__nv_bfloat16*>(q_out);
+    a.k = QuantJob{nullptr, k_scale_exp, k_upper, k_shared, rotate_k ? 1 : 0, 0, 0};
+    a.v = QuantJob{nullptr, v_scale_exp, v_upper, v_shared, 0, 0, 0};
+    a.ld = ld; a.start = start; a.Lcap = Lcap;
+    a.start_per_seq = start_per_seq; a.pos = pos; a.counts = counts;
+    a.q_gain = q_gain; a.k_gain = k_gain; a.gain_f32 = gain_is_f32 ? 1 : 0;
+    a.rope = Rope{rope_cos, rope_sin, rope_rows};
+    a.eps = eps;
+    a.sticky = sticky_status();
+    a.B = (int)B; a.T = (int)T; a.Hq = (int)H; a.Hkv = (int)Hkv;
+    a.wide = !((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 15) && ld % 8 == 0;
+    const bool rows8 = gs == 2 && !((reinterpret_cast<uintptr_t>(k_shared) | reinterpret_cast<uintptr_t>(v_shared)) & 1);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (D) {
+        case 32: return launch_qkv<1>(a, f, rows8, st);
+        case 64: return launch_qkv<2>(a, f, rows8, st);
+        case 128: return launch_qkv<4>(a, f, rows8, st);
+        default: return launch_qkv<8>(a, f, rows8, st);
+    }
+}
+
+extern "C" int msaq_kv_keep(int8_t* k_scale_exp, uint8_t* k_upper, uint8_t* k_shared, int8_t* v_scale_exp, uint8_t* v_upper,
+                            uint8_t* v_shared, const int32_t* path, const int32_t* count, int64_t start,
+                            const int32_t* start_per_seq, int64_t B, int64_t T, int64_t Hkv, int64_t NB, int64_t Lcap, int u,
+                            int gs, void* stream) {
+    const DeviceScope device;
+    Fmt f;
+    if (!k_scale_exp || !k_upper || !k_shared || !v_scale_exp || !v_upper || !v_shared || !path || !count)
+        return fail(MSAQ_ERR_ARG, "null pointer");
+    if (!make_fmt(u, gs, &f)) return fail(MSAQ_ERR_UNSUPPORTED, "unsupported format u=%d gs=%d", u, gs);
+    if (B <= 0 || Hkv <= 0 || NB <= 0 || Lcap <= 0) return fail(MSAQ_ERR_ARG, "B, Hkv, NB and Lcap must be positive");
+    if (T <= 0 || T > KEEP_MAX_T) return fail(MSAQ_ERR_ARG, "a tree has 1 to %d nodes", KEEP_MAX_T);
+    if (Hkv > 65535 || NB > 65535 || B > INT32_MAX / (Hkv * NB)) return fail(MSAQ_ERR_ARG, "size exceeds the supported range");
+    if (!start_per_seq && (start < 0 || start + T > Lcap))
+        return fail(MSAQ_ERR_ARG, "slots [%lld, %lld) exceed the cache capacity %lld", (long long)start, (long long)(start + T), (long long)Lcap);
+    if ((reinterpret_cast<uintptr_t>(k_upper) | reinterpret_cast<uintptr_t>(v_upper)) & 3)
+        return fail(MSAQ_ERR_ARG, "upper planes must be 4-byte aligned");
+    if (int rc = require_sm100()) return rc;
+    const KeepArgs a{{k_scale_exp, v_scale_exp}, {k_upper, v_upper}, {k_shared, v_shared}, path, count, start_per_seq, start, Lcap,
+                     sticky_status(), (int)T, (int)Hkv, (int)NB, f.UB, f.SB, B * Hkv * NB};
+    launch_chained(keep_kernel, dim3((unsigned)((a.planes + 3) / 4), 2), dim3(128), 0, static_cast<cudaStream_t>(stream), a);
+    count_launch();
+    return check_launch("kv_keep");
+}

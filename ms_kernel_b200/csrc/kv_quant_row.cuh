@@ -29,17 +29,13 @@ struct QuantJobs { QuantJob j[2]; };
 constexpr int QROW_CW = 12;                                  // code words per block: 7 of upper codes, then shared codes
 
 // rowbuf: D floats, codes: (D / 32) * QROW_CW words of shared memory owned by the calling warp.
-// head / key: the row's place in the planes ([head][block][key], key stride Lcap); row: its index in job.X.
+// head / key: the row's place in the planes ([head][block][key], key stride Lcap).  v: the row, EPL consecutive values per
+// lane, before the Hadamard rotation.
 template <int EPL>
-__device__ __forceinline__ void quantize_row_warp(const QuantJob& job, const Rope& rope, int64_t row, int64_t head, int64_t key,
-                                                  int64_t Lcap, const Fmt& f, float* rowbuf, uint32_t* codes, int lane) {
+__device__ __forceinline__ void quantize_values_warp(float (&v)[EPL], const QuantJob& job, int64_t head, int64_t key, int64_t Lcap,
+                                                     const Fmt& f, float* rowbuf, uint32_t* codes, int lane) {
     constexpr int D = 32 * EPL, NB = EPL;
     constexpr int CW = QROW_CW;
-    float v[EPL];
-    const __nv_bfloat16* src = job.X + row * D + lane * EPL;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) v[i] = __bfloat162float(src[i]);
-    if (job.rope && rope.cos) rope_warp<EPL>(v, lane, rope, rope.rows == 1 ? 0 : key);
     if (job.rot != 0) {
         fwht_warp<EPL>(v, lane);
         const float inv = (float)(1.0 / sqrt((double)D));
@@ -115,24 +111,27 @@ __device__ __forceinline__ void quantize_row_warp(const QuantJob& job, const Rop
     }
 }
 
+// The same for row `row` of job.X, with the rotary embedding in front where the job asks for it.
+template <int EPL>
+__device__ __forceinline__ void quantize_row_warp(const QuantJob& job, const Rope& rope, int64_t row, int64_t head, int64_t key,
+                                                  int64_t Lcap, const Fmt& f, float* rowbuf, uint32_t* codes, int lane) {
+    constexpr int D = 32 * EPL;
+    float v[EPL];
+    const __nv_bfloat16* src = job.X + row * D + lane * EPL;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) v[i] = __bfloat162float(src[i]);
+    if (job.rope && rope.cos) rope_warp<EPL>(v, lane, rope, rope.rows == 1 ? 0 : key);
+    quantize_values_warp<EPL>(v, job, head, key, Lcap, f, rowbuf, codes, lane);
+}
+
 // The same for the gs = 2 formats with eight consecutive values per lane (quant8.cuh): a warp takes 8 / EPL rows at once,
-// 4 * EPL lanes to a row, and nothing goes through shared memory.  `row`, `head`, `key` and `live` are the lane's row's;
-// lanes of a row that is not live load and store nothing.  job.X must be 16-byte aligned, job.upper 4-, job.shared 2-byte.
+// 4 * EPL lanes to a row, and nothing goes through shared memory.  `head`, `key` and `live` are the lane's row's; lanes of a row
+// that is not live store nothing.  job.upper must be 4-byte, job.shared 2-byte aligned.
 template <int EPL, int U>
-__device__ __forceinline__ void quantize_rows8_warp(const QuantJob& job, const Rope& rope, int64_t row, int64_t head, int64_t key,
-                                                    int64_t Lcap, bool live, int lane) {
+__device__ __forceinline__ void quantize_values8_warp(float (&v)[8], const QuantJob& job, int64_t head, int64_t key, int64_t Lcap,
+                                                      bool live, int lane) {
     constexpr int D = 32 * EPL, NB = EPL, LANES = 4 * EPL, UB = 4 * (8 - U), SB = 2 * U;
     const int l = lane % LANES;
-    float v[8];
-    const uint4 raw = live ? *reinterpret_cast<const uint4*>(job.X + row * D + l * 8) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(w[i]); v[2 * i + 1] = bf16_hi(w[i]); }
-    if (job.rope && rope.cos && live) {
-        const int64_t at = (rope.rows == 1 ? 0 : key) * (D / 2) + l * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rope_pair(v[2 * i], v[2 * i + 1], rope.cos[at + i], rope.sin[at + i], &v[2 * i], &v[2 * i + 1]);
-    }
     if (job.rot != 0) {                                       // the butterfly of fwht_warp, eight values per lane
 #pragma unroll
         for (int h = 1; h < 8; h <<= 1)
@@ -158,6 +157,26 @@ __device__ __forceinline__ void quantize_rows8_warp(const QuantJob& job, const R
     const int64_t slot = (head * NB + (l >> 2)) * Lcap + key;
     quant8_store<U>(c, lane, live, job.upper + slot * UB, job.shared + slot * SB);
     if (live && (lane & 3) == 0) job.scale_exp[slot] = (int8_t)c.e;
+}
+
+// The same for row `row` of job.X (16-byte aligned), with the rotary embedding in front where the job asks for it; lanes of a
+// row that is not live load nothing either.
+template <int EPL, int U>
+__device__ __forceinline__ void quantize_rows8_warp(const QuantJob& job, const Rope& rope, int64_t row, int64_t head, int64_t key,
+                                                    int64_t Lcap, bool live, int lane) {
+    constexpr int D = 32 * EPL, LANES = 4 * EPL;
+    const int l = lane % LANES;
+    float v[8];
+    const uint4 raw = live ? *reinterpret_cast<const uint4*>(job.X + row * D + l * 8) : make_uint4(0u, 0u, 0u, 0u);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(w[i]); v[2 * i + 1] = bf16_hi(w[i]); }
+    if (job.rope && rope.cos && live) {
+        const int64_t at = (rope.rows == 1 ? 0 : key) * (D / 2) + l * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rope_pair(v[2 * i], v[2 * i + 1], rope.cos[at + i], rope.sin[at + i], &v[2 * i], &v[2 * i + 1]);
+    }
+    quantize_values8_warp<EPL, U>(v, job, head, key, Lcap, live, lane);
 }
 
 }  // namespace msaq

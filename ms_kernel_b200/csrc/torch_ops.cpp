@@ -455,6 +455,136 @@ Tensor kv_decode_attention_append(const Tensor& q, const Tensor& k_new, const Te
     return out;
 }
 
+// ---- a step with several drafted tokens ------------------------------------------------------------------------
+const int32_t* opt_int32(const c10::optional<Tensor>& t, int64_t n, const Tensor& like, const char* name) {
+    if (!t.has_value()) return nullptr;
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() == n && t->device() == like.device(), name,
+                " must be a contiguous CUDA int32 tensor of ", n, " elements on the activations' device");
+    return t->data_ptr<int32_t>();
+}
+
+// qkv [B, T, (H + 2 Hkv) D] -> q [B, T, H, D]; keys and values into the planes.  The tokens may lie further apart than their heads.
+Tensor kv_write_qkv(const Tensor& qkv, Tensor ks, Tensor ku, Tensor kh, Tensor vs, Tensor vu, Tensor vh,
+                    const c10::optional<Tensor>& start_t, const c10::optional<Tensor>& pos, const c10::optional<Tensor>& counts,
+                    const c10::optional<Tensor>& q_gain, const c10::optional<Tensor>& k_gain, const c10::optional<Tensor>& cos,
+                    const c10::optional<Tensor>& sin, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t NB,
+                    int64_t start, int64_t Lcap, int64_t u, int64_t gs, bool rotate_k, double eps) {
+    TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == at::kBFloat16, "qkv must be a CUDA bf16 tensor");
+    TORCH_CHECK(B >= 1 && T >= 1 && H >= 1 && Hkv >= 1 && D >= 1, "B, T, H, Hkv and D must be positive");
+    TORCH_CHECK(qkv.dim() == 3 && qkv.size(0) == B && qkv.size(1) == T && qkv.size(2) == (H + 2 * Hkv) * D,
+                "qkv must be [B, T, (H + 2 Hkv) D] = [", B, ", ", T, ", ", (H + 2 * Hkv) * D, "]");
+    const int64_t ld = T > 1 ? qkv.stride(1) : B > 1 ? qkv.stride(0) : qkv.size(2);
+    TORCH_CHECK(qkv.stride(2) == 1 && ld >= qkv.size(2) && (B == 1 || T == 1 || qkv.stride(0) == T * ld),
+                "qkv must have its tokens at one distance and each token's heads side by side");
+    int64_t UB, SB;
+    fmt_sizes(u, gs, &UB, &SB);
+    check_planes(ks, ku, kh, qkv, B * Hkv * NB * Lcap, UB, SB);
+    check_planes(vs, vu, vh, qkv, B * Hkv * NB * Lcap, UB, SB);
+    const int32_t* sp = opt_int32(start_t, B, qkv, "start");
+    const int32_t* pp = opt_int32(pos, B * T, qkv, "pos");
+    const int32_t* cp = opt_int32(counts, B, qkv, "counts");
+    int gain_f32 = -1;
+    const void* gains[2] = {nullptr, nullptr};
+    const c10::optional<Tensor>* given[2] = {&q_gain, &k_gain};
+    for (int i = 0; i < 2; ++i) {
+        if (!given[i]->has_value()) continue;
+        const Tensor& g = **given[i];
+        TORCH_CHECK(g.is_cuda() && g.device() == qkv.device() && g.is_contiguous() && g.numel() == D &&
+                    (g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16),
+                    "gains must be contiguous bf16 or fp32 tensors of D elements on the activations' device");
+        const int f32 = g.scalar_type() == at::kFloat;
+        TORCH_CHECK(gain_f32 < 0 || gain_f32 == f32, "q_gain and k_gain must have one type");
+        gain_f32 = f32;
+        gains[i] = g.data_ptr();
+    }
+    TORCH_CHECK(cos.has_value() == sin.has_value(), "cos and sin come together");
+    if (cos.has_value()) check_rope(*cos, *sin, qkv, D);
+    c10::cuda::CUDAGuard guard(qkv.device());
+    Tensor q = at::empty({B, T, H, D}, qkv.options());
+    check_rc(msaq_kv_write_qkv(qkv.data_ptr(), ld, q.data_ptr(), ks.data_ptr<int8_t>(), ku.data_ptr<uint8_t>(), kh.data_ptr<uint8_t>(),
+                               vs.data_ptr<int8_t>(), vu.data_ptr<uint8_t>(), vh.data_ptr<uint8_t>(), B, T, H, Hkv, D, NB, start, sp,
+                               pp, cp, gains[0], gains[1], gain_f32 == 1, eps, cos.has_value() ? cos->data_ptr<float>() : nullptr,
+                               sin.has_value() ? sin->data_ptr<float>() : nullptr, cos.has_value() ? cos->size(0) : 0, Lcap, (int)u,
+                               (int)gs, rotate_k ? 1 : 0, stream_of(qkv)),
+             "kv_write_qkv");
+    return q;
+}
+
+Tensor kv_tree_attention(const Tensor& q, const Tensor& ks, const Tensor& ku, const Tensor& kh, const Tensor& vs, const Tensor& vu,
+                         const Tensor& vh, const Tensor& mask, const c10::optional<Tensor>& lens, int64_t Hkv, int64_t Lk, int64_t D,
+                         int64_t NB, int64_t u, int64_t gs, int64_t Lcap, bool qrot) {
+    check_act(q, "q");
+    TORCH_CHECK(q.dim() == 4 && q.size(3) == D && q.numel() > 0, "q must be [B, T, H, D]");
+    const int64_t B = q.size(0), T = q.size(1), H = q.size(2);
+    reject_numeric_toggles();
+    int64_t UB, SB;
+    fmt_sizes(u, gs, &UB, &SB);
+    TORCH_CHECK(mask.is_cuda() && mask.scalar_type() == at::kLong && mask.is_contiguous() && mask.device() == q.device() &&
+                ((mask.dim() == 1 && mask.size(0) == T) || (mask.dim() == 2 && mask.size(0) == B && mask.size(1) == T)),
+                "mask must be a contiguous CUDA int64 tensor [T] or [B, T] on the activations' device");
+    check_planes(ks, ku, kh, q, B * Hkv * NB * Lcap, UB, SB);
+    check_planes(vs, vu, vh, q, B * Hkv * NB * Lcap, UB, SB);
+    const int32_t* lp = opt_int32(lens, B, q, "lens");
+    c10::cuda::CUDAGuard guard(q.device());
+    Tensor out = at::empty_like(q);
+    const size_t wsb = msaq_kv_tree_workspace(B, T, H, Hkv, Lk, D);
+    Tensor ws = workspace(q, wsb);
+    check_rc(msaq_kv_tree_attention(q.data_ptr(), ks.data_ptr<int8_t>(), ku.data_ptr<uint8_t>(), kh.data_ptr<uint8_t>(),
+                                    vs.data_ptr<int8_t>(), vu.data_ptr<uint8_t>(), vh.data_ptr<uint8_t>(), out.data_ptr(), nullptr, lp,
+                                    reinterpret_cast<const uint64_t*>(mask.data_ptr<int64_t>()), mask.dim() == 2 ? T : 0, B, T, H, Hkv,
+                                    Lk, D, NB, (int)u, (int)gs, Lcap, qrot ? 1 : 0, ws.data_ptr(), wsb, stream_of(q)),
+             "kv_tree_attention");
+    return out;
+}
+
+std::vector<Tensor> verify_tree(const Tensor& target, const Tensor& tokens, const Tensor& parents, const Tensor& uniforms,
+                                const c10::optional<Tensor>& draft) {
+    TORCH_CHECK(target.is_cuda() && target.dim() == 3 && target.numel() > 0 &&
+                (target.scalar_type() == at::kFloat || target.scalar_type() == at::kBFloat16),
+                "target_probs must be a CUDA fp32 or bf16 tensor [B, T, V]");
+    const int64_t B = target.size(0), T = target.size(1), V = target.size(2);
+    TORCH_CHECK(V == 1 || target.stride(2) == 1, "target_probs must have its vocabulary side by side");
+    if (draft.has_value())
+        TORCH_CHECK(draft->device() == target.device() && draft->scalar_type() == target.scalar_type() && draft->sizes() == target.sizes() &&
+                    (V == 1 || draft->stride(2) == 1), "draft_probs must have the shape, type and device of target_probs and its vocabulary side by side");
+    auto whole = [&](const Tensor& t, at::ScalarType ty) { return t.device() == target.device() && t.scalar_type() == ty && t.is_contiguous(); };
+    TORCH_CHECK(whole(tokens, at::kInt) && tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == T,
+                "tokens must be a contiguous int32 tensor [B, T] on the probabilities' device");
+    TORCH_CHECK(whole(parents, at::kInt) && ((parents.dim() == 1 && parents.size(0) == T) ||
+                (parents.dim() == 2 && parents.size(0) == B && parents.size(1) == T)),
+                "parents must be a contiguous int32 tensor [T] or [B, T] on the probabilities' device");
+    TORCH_CHECK(whole(uniforms, at::kFloat) && uniforms.dim() == 2 && uniforms.size(0) == B && uniforms.size(1) == T,
+                "uniforms must be a contiguous fp32 tensor [B, T] on the probabilities' device");
+    c10::cuda::CUDAGuard guard(target.device());
+    Tensor path = at::empty({B, T}, tokens.options()), count = at::empty({B}, tokens.options()), token = at::empty({B}, tokens.options());
+    check_rc(msaq_verify_tree(target.data_ptr(), target.stride(0), target.stride(1), draft.has_value() ? draft->data_ptr() : nullptr,
+                              draft.has_value() ? draft->stride(0) : 0, draft.has_value() ? draft->stride(1) : 0,
+                              target.scalar_type() == at::kFloat, tokens.data_ptr<int32_t>(), parents.data_ptr<int32_t>(),
+                              parents.dim() == 2 ? T : 0, uniforms.data_ptr<float>(), path.data_ptr<int32_t>(), count.data_ptr<int32_t>(),
+                              token.data_ptr<int32_t>(), B, T, V, stream_of(target)),
+             "verify_tree");
+    return {path, count, token};
+}
+
+void kv_keep(Tensor ks, Tensor ku, Tensor kh, Tensor vs, Tensor vu, Tensor vh, const Tensor& path, const Tensor& count,
+             const c10::optional<Tensor>& start_t, int64_t Hkv, int64_t NB, int64_t start, int64_t Lcap, int64_t u, int64_t gs) {
+    TORCH_CHECK(path.is_cuda() && path.scalar_type() == at::kInt && path.is_contiguous() && path.dim() == 2 && path.numel() > 0,
+                "path must be a contiguous CUDA int32 tensor [B, T]");
+    const int64_t B = path.size(0), T = path.size(1);
+    TORCH_CHECK(count.device() == path.device() && count.scalar_type() == at::kInt && count.is_contiguous() && count.numel() == B,
+                "count must be a contiguous int32 tensor of B elements on path's device");
+    int64_t UB, SB;
+    fmt_sizes(u, gs, &UB, &SB);
+    check_planes(ks, ku, kh, path, B * Hkv * NB * Lcap, UB, SB);
+    check_planes(vs, vu, vh, path, B * Hkv * NB * Lcap, UB, SB);
+    const int32_t* sp = opt_int32(start_t, B, path, "start");
+    c10::cuda::CUDAGuard guard(path.device());
+    check_rc(msaq_kv_keep(ks.data_ptr<int8_t>(), ku.data_ptr<uint8_t>(), kh.data_ptr<uint8_t>(), vs.data_ptr<int8_t>(),
+                          vu.data_ptr<uint8_t>(), vh.data_ptr<uint8_t>(), path.data_ptr<int32_t>(), count.data_ptr<int32_t>(), start, sp,
+                          B, T, Hkv, NB, Lcap, (int)u, (int)gs, stream_of(path)),
+             "kv_keep");
+}
+
 // x [B, heads, D] bf16 -> RoPE at position pos (pos_t[b] per sequence when given).
 Tensor rope(const Tensor& x, const Tensor& cos, const Tensor& sin, const c10::optional<Tensor>& pos_t, int64_t pos) {
     check_act(x, "x");
@@ -867,6 +997,14 @@ TORCH_LIBRARY(msaq, m) {
           "int OUT, int NB, int u, int gs, int[] peer_ptrs, int rank, int parity) -> ()", &wonly_gemv_fused_push);
     m.def("peer_exchange_recv(Tensor like, Tensor? residual, int[] peer_ptrs, int rank, int parity, int M, int OUT) -> Tensor",
           &peer_exchange_recv);
+    m.def("kv_write_qkv(Tensor qkv, Tensor(a!) ks, Tensor(b!) ku, Tensor(c!) kh, Tensor(d!) vs, Tensor(e!) vu, Tensor(f!) vh, "
+          "Tensor? start_t, Tensor? pos, Tensor? counts, Tensor? q_gain, Tensor? k_gain, Tensor? cos, Tensor? sin, int B, int T, int H, "
+          "int Hkv, int D, int NB, int start, int Lcap, int u, int gs, bool rotate_k, float eps) -> Tensor", &kv_write_qkv);
+    m.def("kv_tree_attention(Tensor q, Tensor ks, Tensor ku, Tensor kh, Tensor vs, Tensor vu, Tensor vh, Tensor mask, Tensor? lens, "
+          "int Hkv, int Lk, int D, int NB, int u, int gs, int Lcap, bool qrot) -> Tensor", &kv_tree_attention);
+    m.def("verify_tree(Tensor target_probs, Tensor tokens, Tensor parents, Tensor uniforms, Tensor? draft_probs) -> Tensor[]", &verify_tree);
+    m.def("kv_keep(Tensor(a!) ks, Tensor(b!) ku, Tensor(c!) kh, Tensor(d!) vs, Tensor(e!) vu, Tensor(f!) vh, Tensor path, Tensor count, "
+          "Tensor? start_t, int Hkv, int NB, int start, int Lcap, int u, int gs) -> ()", &kv_keep);
     m.def("launch_count() -> int", &launch_count);
     m.def("set_option(int option, int value) -> ()", &set_option);
     m.def("get_option(int option) -> int", &get_option);

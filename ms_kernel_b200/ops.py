@@ -247,6 +247,81 @@ class KVCache:
                                                *self.k, *self.v, seq_lens, self.B, Hq, self.Hkv, Lk, self.D, self.nb, self.u,
                                                self.gs, self.Lcap, self.rotate, self.rotate, cos, sin, pos_t, pos_i)
 
+    # ---- a step with several drafted tokens (include/msaq_b200.h: "a step with several drafted tokens") ----
+    def write_qkv(self, qkv, Hq, start, rope=None, q_gain=None, k_gain=None, eps=1e-6, pos=None, counts=None):
+        """The QKV projection's output to attention: queries normed and rotated, keys normed, rotated and quantised, values
+        quantised, in one launch.
+
+        qkv [B,T,(Hq+2Hkv)*D] bf16 (tokens may lie further apart than their heads) -> q [B,T,Hq,D] bf16; the keys and
+        values go to slots start + t (start: int, or int32 tensor [B]).  q_gain, k_gain [D] bf16 or fp32: RMS norm of each
+        head with that gain, None: no norm.  rope = (cos, sin) fp32 [rows,D/2], indexed by pos (int32 [B,T]; default: the
+        slots).  counts int32 [B]: how many of a sequence's T tokens are there; the query rows of the others are 0 and
+        their slots stay.  T is any length, one token to a prompt."""
+        B, T = int(qkv.shape[0]), int(qkv.shape[1])
+        start_t, start_i = (None, int(start)) if isinstance(start, int) else (start, 0)
+        cos, sin = (None, None) if rope is None else (rope[0], rope[1])
+        return _OPS.kv_write_qkv(qkv, *self.k, *self.v, start_t, pos, counts, q_gain, k_gain, cos, sin, B, T, int(Hq), self.Hkv,
+                                 self.D, self.nb, start_i, self.Lcap, self.u, self.gs, self.rotate, float(eps))
+
+    def attend_tree(self, q, mask, Lk, lens=None):
+        """q [B,T,Hq,D] bf16, T <= 64 nodes of a tree per sequence, node i in slot lens[b] + i -> [B,T,Hq,D] bf16.
+
+        Node i attends the keys [0, lens[b]) and slot lens[b] + j for every bit j of mask[b,i] (int64 [B,T], or [T] for one tree
+        for all: see tree_mask); a node that attends nothing gives 0.  Lk: keys that any sequence can attend, the nodes included;
+        lens int32 [B], default Lk - T."""
+        if int(q.shape[0]) != self.B:
+            raise ValueError("q has %d sequences, the cache %d" % (int(q.shape[0]), self.B))
+        return _OPS.kv_tree_attention(q, *self.k, *self.v, mask, lens, self.Hkv, int(Lk), self.D, self.nb, self.u, self.gs, self.Lcap,
+                                      self.rotate)
+
+    def keep(self, start, path, count):
+        """After verify_tree: slot start + k takes what slot start + path[b,k] held, k < count[b] (start: int, or int32 tensor
+        [B]); all other slots stay.  The cache then holds the accepted nodes behind each other."""
+        if int(path.shape[0]) != self.B:
+            raise ValueError("path has %d sequences, the cache %d" % (int(path.shape[0]), self.B))
+        start_t, start_i = (None, int(start)) if isinstance(start, int) else (start, 0)
+        _OPS.kv_keep(*self.k, *self.v, path, count, start_t, self.Hkv, self.nb, start_i, self.Lcap, self.u, self.gs)
+
+
+# --------------------------------------------------------------------------
+# trees of drafted tokens
+# --------------------------------------------------------------------------
+def tree_mask(parents, device="cuda"):
+    """Parents of a tree's nodes ([T] or [B,T] whole numbers on the host; -1: the root, and nodes that are not there) -> (mask int64,
+    depth int32) of the same shape on `device`: bit j of mask[..., i] says that node i attends node j (itself and its
+    ancestors; none for a node that is not there), depth counts from the root."""
+    import numpy as np
+    par = np.asarray(parents, dtype=np.int64)
+    T = par.shape[-1]
+    if par.ndim not in (1, 2) or not 1 <= T <= 64:
+        raise ValueError("parents must be [T] or [B, T] with 1 to 64 nodes")
+    rows = par.reshape(-1, T)
+    if (rows[:, 0] != -1).any() or (rows >= np.arange(T)).any() or (rows < -1).any():
+        raise ValueError("node 0 is the root (-1), every other node's parent is in front of it or -1")
+    mask, depth = np.zeros(rows.shape, np.uint64), np.zeros(rows.shape, np.int32)
+    mask[:, 0] = 1
+    b = np.arange(rows.shape[0])
+    for i in range(1, T):
+        p = rows[:, i]
+        there = (p >= 0) & (mask[b, p] != 0)               # a node under one that is not there is not there either
+        mask[:, i] = np.where(there, mask[b, p] | np.uint64(1 << i), 0)
+        depth[:, i] = np.where(there, depth[b, p] + 1, 0)
+    return (torch.from_numpy(mask.view(np.int64).reshape(par.shape)).to(device),
+            torch.from_numpy(depth.reshape(par.shape)).to(device))
+
+
+def verify_tree(target_probs, tokens, parents, uniforms, draft_probs=None):
+    """Which drafted tokens stay (recursive rejection sampling; include/msaq_b200.h: msaq_verify_tree).
+
+    target_probs [B,T,V] fp32 or bf16: the target's distribution behind each node; draft_probs (same shape and type): row i is
+    the distribution that node i's children were drawn from, None: the children were chosen, not drawn.  tokens int32 [B,T];
+    parents int32 [B,T] or [T]; uniforms fp32 [B,T] in [0,1): a node's random number (entry 0: the final draw's).
+    -> path int32 [B,T] (accepted nodes, the root first, then -1), count int32 [B] (the root included), token int32 [B] (the one
+    behind them: the next root)."""
+    _require()
+    path, count, token = _OPS.verify_tree(target_probs, tokens, parents, uniforms, draft_probs)
+    return path, count, token
+
 
 # --------------------------------------------------------------------------
 # plain MXINT8 twins (the reference's matched baseline format, ms_lib/pack.py:530-594)
