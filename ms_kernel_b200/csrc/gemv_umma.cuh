@@ -35,6 +35,7 @@
 #pragma once
 
 #include "gemv_mma.cuh"
+#include "tcgen05.cuh"
 
 namespace msaq {
 
@@ -55,67 +56,6 @@ __host__ __device__ constexpr int gu_sb(int u) { return 2 * u; }
 __host__ __device__ constexpr int gu_packed(int u) { return GU_TR * (gu_ub(u) + gu_sb(u) + 1); }   // packed bytes of a unit
 __host__ __device__ constexpr int gu_stage(int u) { return gu_packed(u) + GU_XTILE; }
 constexpr int GU_TMEM_COLS = GU_TR;                // one fp32 accumulator column per weight row of the tile
-
-// ---- tcgen05 wrappers -----------------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// Arrive on `bar` once every tcgen05 operation this thread issued so far has completed.
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// D[tmem] (+)= A[smem desc] * B[smem desc]; accumulate == 0 overwrites D.  The two matrix
-// descriptors arrive as 32-bit halves: the upper half is the same for every MMA of the kernel,
-// the lower half moves with the operand's address, so the issuing thread spends one add per operand.
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc,
-                                         uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 da, {%1, %3};\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// 16 consecutive accumulator columns of this warp's 32 lanes.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// Shared-memory matrix descriptor, K-major, no swizzle: 8-row x 16-byte core matrices of 128
-// contiguous bytes; `lbo` is the byte distance between core matrices adjacent in K, `sbo`
-// between core matrices adjacent in the row direction.  Bits 46-47 = 1: sm_100 descriptor.
-__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t saddr, uint32_t lbo) {
-    return ((saddr >> 4) & 0x3FFFu) | (((lbo >> 4) & 0x3FFFu) << 16);
-}
-__device__ __forceinline__ uint32_t umma_desc_hi(uint32_t sbo) { return ((sbo >> 4) & 0x3FFFu) | (1u << 14); }
-// Instruction descriptor of kind::f16: fp32 accumulator, bf16 A and B, both K-major, M = 128, N = n.
-__host__ __device__ inline uint32_t umma_idesc_bf16(int n) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-
-__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
 
 // ---- activation staging ----------------------------------------------------------
 // X [M][K] bf16 row-major -> per K block the first ceil(M/8) row groups of an A-operand tile in the
@@ -192,14 +132,6 @@ __device__ __forceinline__ void gu_decode_row<4>(uint32_t st, int r, uint32_t ds
     }
 }
 
-// Bits [32*i, 32*i+32) of the pattern that has the top bit of every `width`-bit field set.
-__host__ __device__ constexpr uint32_t gu_sign_pattern(int width, int i) {
-    uint32_t p = 0;
-    for (int b = width - 1; b < 32 * (i + 1); b += width)
-        if (b >= 32 * i) p |= 1u << (b - 32 * i);
-    return p;
-}
-
 // u = 3 (5-bit upper, 3-bit shared) and u = 2 (6-bit, 2-bit): fields cut out of the dense bit runs
 // with funnel shifts.
 template <int U>
@@ -219,7 +151,7 @@ __device__ __forceinline__ void gu_decode_row(uint32_t st, int r, uint32_t dst) 
         }
     }
 #pragma unroll
-    for (int i = 0; i < NW; ++i) w[i] ^= gu_sign_pattern(WB, i);
+    for (int i = 0; i < NW; ++i) w[i] ^= field_signs(WB, i);
     w[NW] = 0u;
     uint32_t s0, s1 = 0u;                                       // shared run: 16 fields of U bits
     const uint32_t sbase = st + GU_TR * gu_ub(U) + r * gu_sb(U);
@@ -233,8 +165,8 @@ __device__ __forceinline__ void gu_decode_row(uint32_t st, int r, uint32_t dst) 
         s0 = a | (b << 16);
         s1 = c;
     }
-    s0 ^= gu_sign_pattern(U, 0);
-    s1 ^= gu_sign_pattern(U, 1) & 0xFFFFu;
+    s0 ^= field_signs(U, 0);
+    s1 ^= field_signs(U, 1) & 0xFFFFu;
     const int e = lds_s8<0>(st + GU_TR * (gu_ub(U) + gu_sb(U)) + r);
     const float sc = __int_as_float(max(0, e + 127) << 23);
     const float off = -(8388608.0f + 128.0f + (float)(1 << (U - 1))) * sc;

@@ -39,14 +39,14 @@ struct VerifyArgs {
     bool p_vec, q_vec;                       // rows can be read four elements at a time
 };
 
-__device__ __forceinline__ float vf_load(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float vf_load(const float* p) { return *p; }
 __device__ __forceinline__ float vf_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void vf_load4(const float* p, float (&v)[4]) {
-    const float4 t = __ldg(reinterpret_cast<const float4*>(p));
+    const float4 t = *reinterpret_cast<const float4*>(p);
     v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
 }
 __device__ __forceinline__ void vf_load4(const __nv_bfloat16* p, float (&v)[4]) {
-    const uint2 t = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
     v[0] = bf16_lo(t.x); v[1] = bf16_hi(t.x); v[2] = bf16_lo(t.y); v[3] = bf16_hi(t.y);
 }
 // Entries that are not positive and finite count as nothing.

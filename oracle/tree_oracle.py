@@ -63,12 +63,12 @@ def write_qkv(qkv, planes_k, planes_v, Hq, Hkv, D, u, gs, start, tables, q_gain,
 
 
 def tree_attention(q, planes_k, planes_v, u, gs, lens, seen, rotate):
-    """q [B,T,Hq,D]; seen[b][i]: nodes that node i attends -> (out, weight, score) in 64 bits: the result, the same
-    average of |v|, and per (b, i, head) the largest sum |q_d k_d| / sqrt(D) over the attended keys."""
+    """q [B,T,Hq,D]; seen[b][i]: nodes that node i attends -> (out, mag, big, all) in 64 bits: the result, the same
+    average of |v|, per (b, i, head) the largest sum |q_d k_d| / sqrt(D) over the attended keys, and the plain sum of |v| over them."""
     B, T, Hq, D = q.shape
     Hkv = planes_k[0].shape[1]
     G = Hq // Hkv
-    out, mag, big = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:3])
+    out, mag, big, all_v = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:3]), np.zeros(q.shape)
     for b in range(B):
         need = lens[b] + T
         K = orc.dequant_kv_planes(*[p[b][:, :, :need] for p in planes_k], u, gs).astype(np.float64)
@@ -84,8 +84,9 @@ def tree_attention(q, planes_k, planes_v, u, gs, lens, seen, rotate):
                 p = np.exp(s - s.max())
                 p /= p.sum()
                 out[b, i, h], mag[b, i, h] = p @ v, p @ np.abs(v)
+                all_v[b, i, h] = np.abs(v).sum(0)
                 big[b, i, h] = (np.abs(k) @ np.abs(qi[h])).max() / np.sqrt(D)
-    return out, mag, big
+    return out, mag, big, all_v
 
 
 def _clean(p):

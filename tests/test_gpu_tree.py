@@ -148,11 +148,14 @@ def test_write_norm_of_extreme_rows(rng):
 
 
 # ------------------------------------------------------------------------------------------------ attend_tree
-def _bound(ref, mag, big, p_step):
+def _bound(ref, mag, big, all_v, p_step):
     """Elementwise bound of the output's error, relative steps of half a unit: the result's rounding to bf16 (2^-8 of it); of a
     probability (p_step: 2^-11 in fp16, 2^-8 in bf16) and, twice -- numerator and denominator --, what a score is off by: a
-    query element is held in fp16 at least (2^-11), which moves a score by 2^-11 sum |q_d k_d| / sqrt(D) at most; and 2^-18 for sums in 32 bits."""
-    return 2.0 ** -8 * np.abs(ref) + mag * (2 * p_step + 2 * 2.0 ** -11 * big[..., None] + 2.0 ** -18 * (1 + big[..., None])) + 1e-30
+    query element is held in fp16 at least (2^-11), which moves a score by 2^-11 sum |q_d k_d| / sqrt(D) at most; and 2^-18 for sums in 32 bits.
+    fp16 ends: its smallest number is 2^-24, so a probability held times 2^7 relative to the largest one (or to one up to 2^8 smaller) is
+    off by up to 2^-25 / 2^7 = 2^-32 of the largest, whatever its own size; the largest is at most the sum of all, so the average moves by
+    2^-32 sum |v| at most."""
+    return 2.0 ** -8 * np.abs(ref) + mag * (2 * p_step + 2 * 2.0 ** -11 * big[..., None] + 2.0 ** -18 * (1 + big[..., None])) + 2.0 ** -32 * all_v + 1e-30
 
 
 def _attend_case(rng, B, T, Hq, Hkv, D, u, gs, lens, Lcap, rotate=True, seen=None, shared=False, scale=1.0, edit=None, p_step=2.0 ** -11):
@@ -178,10 +181,10 @@ def _attend_case(rng, B, T, Hq, Hkv, D, u, gs, lens, Lcap, rotate=True, seen=Non
     mask = torch.from_numpy(words[0] if shared else words).cuda()
     q = orc.to_bf16(rng.standard_normal((B, T, Hq, D)).astype(np.float32) * scale)
     got = c.attend_tree(_bf(q), mask, Lk, _i32(lens)).float().cpu().numpy()
-    ref, mag, big = tro.tree_attention(q, _planes(c.k), _planes(c.v), u, gs, lens, seen, rotate)
+    ref, mag, big, all_v = tro.tree_attention(q, _planes(c.k), _planes(c.v), u, gs, lens, seen, rotate)
     assert np.isfinite(got).all()
     err = np.abs(got - ref)
-    lim = _bound(ref, mag, big, p_step)
+    lim = _bound(ref, mag, big, all_v, p_step)
     assert (err <= lim).all(), "worst %.3f of the bound" % (err / lim).max()
     return c, q, mask, Lk, got
 
@@ -257,8 +260,8 @@ def test_attend_infinities_in_unseen_nodes(rng, u, gs):
     for pl in (*pk, *pv):
         pl[:, :, :, 45 + bad] = 0                              # not attended by these rows: any finite value will do
     keep = [[s if bad not in s else set() for s in seen[0]]]
-    ref, mag, big = tro.tree_attention(q, pk, pv, u, gs, lens, keep, True)
-    lim = _bound(ref, mag, big, 2.0 ** -8)
+    ref, mag, big, all_v = tro.tree_attention(q, pk, pv, u, gs, lens, keep, True)
+    lim = _bound(ref, mag, big, all_v, 2.0 ** -8)
     assert np.isfinite(got[:, rows]).all()
     assert (np.abs(got - ref)[:, rows] <= lim[:, rows]).all()
 
@@ -634,3 +637,18 @@ def test_calls_on_two_streams_do_not_meet(rng):
     for i, (a, v) in enumerate(outs):
         assert np.array_equal(a.float().cpu().numpy(), jobs[i % 2][4])
         assert all(torch.equal(x, y) for x, y in zip(v, want))
+
+
+def test_attend_gives_up_and_recovers(rng):
+    """A product whose completion is never signalled: the waits run out, the rows are NaN, the status word says so, and the next call is
+    right."""
+    import cabi
+    c, q, mask, Lk, got = _attend_case(rng, 1, 8, 8, 1, 128, 4, 2, np.array([1000]), 1008)
+    _status()
+    with cabi.options({3: 4096, 4: 0}):
+        bad = c.attend_tree(_bf(q), mask, Lk)
+        torch.cuda.synchronize()
+    assert _status() == 4
+    assert torch.isnan(bad).all()
+    assert np.array_equal(c.attend_tree(_bf(q), mask, Lk).float().cpu().numpy(), got)
+    assert _status() == 0
