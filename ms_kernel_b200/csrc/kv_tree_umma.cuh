@@ -22,6 +22,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "tcgen05.cuh"
 #include "kv_tree_generic.cuh"
 
@@ -166,12 +168,11 @@ __device__ __forceinline__ bool ktu_zero(const KtuRaw<2>& r) {
 // numbers 1024 + ...  Order inside the eight: U = 4: 0 2, 4 6, 1 3, 5 7 (ktu_place), else as they are.
 template <int U> __device__ __forceinline__ void ktu_codes(const KtuRaw<U>& r, int i, uint32_t (&w)[4]);
 template <> __device__ __forceinline__ void ktu_codes<4>(const KtuRaw<4>& r, int i, uint32_t (&w)[4]) {
-    const uint32_t x = (i == 0 ? r.u.x : i == 1 ? r.u.y : i == 2 ? r.u.z : r.u.w) ^ 0x88888888u;
-    const uint32_t s = (i < 2 ? r.s.x : r.s.y) ^ 0x88888888u;
-    // the four shared codes of these elements (two elements each), one per byte
+    const uint32_t x = i == 0 ? r.u.x : i == 1 ? r.u.y : i == 2 ? r.u.z : r.u.w, s = i < 2 ? r.s.x : r.s.y;
+    // the four shared codes of these elements (two elements each), one per byte; the sign bits of both codes flipped on the way
     const uint32_t t = prmt(s, 0u, (i & 1) ? 0x3322u : 0x1100u);
-    const uint32_t lo = and_or(t >> 4, 0x0F000F00u, t & 0x000F000Fu);
-    const uint32_t e = and_or(x << 4, 0xF0F0F0F0u, lo), o = and_or(x, 0xF0F0F0F0u, lo);
+    const uint32_t lo = and_xor(t >> 4, 0x0F000F00u, and_xor(t, 0x000F000Fu, 0x88888888u));
+    const uint32_t e = and_xor(x << 4, 0xF0F0F0F0u, lo), o = and_xor(x, 0xF0F0F0F0u, lo);
     w[0] = prmt(e, 0x64646464u, 0x4140u);
     w[1] = prmt(e, 0x64646464u, 0x4342u);
     w[2] = prmt(o, 0x64646464u, 0x4140u);
@@ -231,6 +232,7 @@ kv_tree_umma_kernel(const KvTreeArgs a) {
     uint8_t* const smem = ktu_smem_raw + (sbase - smem_u32(ktu_smem_raw));
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3, half = warp >> 2;
+    const bool issuer = __shfl_sync(0xffffffffu, warp, 0) == 0;    // the warp that issues the MMAs
     const int key = quad * 32 + lane;                             // this thread's key of a tile; its blocks are 2 half, 2 half + 1
     const int groups = gridDim.y / a.Hkv, hk = blockIdx.y / groups, grp = blockIdx.y % groups, b = blockIdx.z;
     const int G = a.Hq / a.Hkv, R = a.T * G, r0 = grp * NR, rows = min(NR, R - r0);
@@ -356,7 +358,7 @@ kv_tree_umma_kernel(const KvTreeArgs a) {
         ktu_st_wait();
         tc_fence_before();
         const bool wide = __syncthreads_or(far);
-        if (tid == 0) {
+        if (issuer && elect_lane()) {
             tc_fence_after();
             const uint32_t bhi = ktu_desc_hi(1024);
 #pragma unroll
@@ -415,7 +417,6 @@ kv_tree_umma_kernel(const KvTreeArgs a) {
             }
         }
         float x[NC];
-        bool move = it == 0;
 #pragma unroll
         for (int c = 0; c < NC; c += 8) {
             ktu_ld8(tlane + KTU_COL_S + half * NC + c, &x[c]);
@@ -423,10 +424,16 @@ kv_tree_umma_kernel(const KvTreeArgs a) {
             for (int k = 0; k < 8; ++k) {
                 const float2 rf = ref[half * NC + c + k];
                 x[c + k] = fmaf(x[c + k] * ck, rf.x, rf.y);
-                if (tail && !(vis >> (c + k) & 1)) x[c + k] = -INFINITY;
-                move = move || x[c + k] > KTU_MOVE;
             }
         }
+        if (tail)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (!(vis >> c & 1)) x[c] = -INFINITY;
+        float top = x[0];
+#pragma unroll
+        for (int c = 1; c < NC; ++c) top = fmaxf(top, x[c]);
+        const bool move = it == 0 || top > KTU_MOVE;
         if (__syncthreads_or(move)) {
             // ---- references move: rows whose maximum of this tile is beyond theirs ----
 #pragma unroll 1
@@ -482,19 +489,23 @@ kv_tree_umma_kernel(const KvTreeArgs a) {
             ktu_st_wait();
         }
         // ---- probabilities to shared memory ----
+        auto store_p = [&](auto bf16) {
 #pragma unroll
-        for (int c = 0; c < NC; c += 8) {
-            uint32_t w[4];
+            for (int c = 0; c < NC; c += 8) {
+                uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 8; k += 2) {
-                const float p0 = ktu_exp2(x[c + k]), p1 = ktu_exp2(x[c + k + 1]);
-                l[c + k] += p0;
-                l[c + k + 1] += p1;
-                if (!wide) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
-                else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
+                for (int k = 0; k < 8; k += 2) {
+                    const float p0 = ktu_exp2(x[c + k]), p1 = ktu_exp2(x[c + k + 1]);
+                    l[c + k] += p0;
+                    l[c + k + 1] += p1;
+                    if constexpr (!decltype(bf16)::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
+                    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
+                }
+                sts128(sbase + KTU_P + (key >> 3) * 1024 + (key & 7) * 128 + (((half * (NC / 8) + c / 8) ^ (key & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
-            sts128(sbase + KTU_P + (key >> 3) * 1024 + (key & 7) * 128 + (((half * (NC / 8) + c / 8) ^ (key & 7)) << 4), w[0], w[1], w[2], w[3]);
-        }
+        };
+        if (wide) store_p(std::true_type{});
+        else store_p(std::false_type{});
         fence_async_smem();
         tc_fence_before();
         const bool give_up = __syncthreads_or(!ok);
@@ -502,7 +513,7 @@ kv_tree_umma_kernel(const KvTreeArgs a) {
             ok = false;
             break;
         }
-        if (tid == 0) {
+        if (issuer && elect_lane()) {
             tc_fence_after();
             const uint32_t hi = ktu_desc_hi(1024), id = ktu_idesc(NR, wide ? 1u : 0u, 1u);
 #pragma unroll
