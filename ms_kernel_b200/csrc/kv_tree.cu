@@ -15,29 +15,20 @@ struct TreePlan {
 // The tuned kernel: head_dim 128, gs = 2, planes on 16-byte boundaries.
 bool umma_eligible(int64_t D, int gs) { return D == 128 && gs == 2; }
 
-// Rows per thread block by the rows there are; key pieces until every SM has its two thread blocks, and up to four times as
-// many where that leaves a piece 1024 keys (queries, first loads and the merge are a fixed cost of a piece).
+// Rows per thread block by the rows there are; as many runs of the line of tiles as there are SMs, or as
+// there can be tiles.
 TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
     TreePlan p;
     const int64_t R = T * (H / Hkv);
     p.rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
     p.groups = (int)((R + p.rows - 1) / p.rows);
-    const int64_t blocks = B * Hkv * p.groups, slots = 2LL * sm_count();
-    int64_t want = (4 * slots + blocks - 1) / blocks;
-    const int64_t most = (Lk + KTU_KEYS - 1) / KTU_KEYS;
-    int64_t one_wave = slots / blocks;
-    if (one_wave > most) one_wave = most;
-    const int64_t cap = Lk / 1024 > one_wave ? Lk / 1024 : one_wave;
-    if (want > cap) want = cap;
-    if (want < 1) want = 1;
-    const int64_t tile = ((Lk + want - 1) / want + KTU_KEYS - 1) / KTU_KEYS * KTU_KEYS;
-    p.key_tile = (int)tile;
-    p.S = (int)((Lk + tile - 1) / tile);
+    p.S = (int)std::min<int64_t>(sm_count(), B * Hkv * p.groups * ((Lk + KTU_KEYS - 1) / KTU_KEYS));
+    p.key_tile = KTU_KEYS;
     return p;
 }
 
 template <int U, int NR>
-int launch_tree_umma_rows(const KvTreeArgs& a, const TreePlan& p, int B, cudaStream_t st) {
+int launch_tree_umma_rows(const KvTreeArgs& a, const TreePlan& p, int B, __nv_bfloat16* out, float* out_f32, cudaStream_t st) {
     static bool configured[64] = {};
     constexpr int smem = ktu_smem_bytes(NR);
     const int dev = current_device();
@@ -46,15 +37,19 @@ int launch_tree_umma_rows(const KvTreeArgs& a, const TreePlan& p, int B, cudaStr
             return fail(MSAQ_ERR_CUDA, "cannot reserve %d bytes of shared memory", smem);
         configured[dev] = true;
     }
-    launch_chained(kv_tree_umma_kernel<U, NR>, dim3((unsigned)p.S, (unsigned)(a.Hkv * p.groups), (unsigned)B), dim3(KTU_THREADS), smem, st, a);
+    launch_chained(kv_tree_umma_kernel<U, NR>, dim3((unsigned)p.S), dim3(KTU_THREADS), smem, st, a, B, p.groups, out, out_f32);
     count_launch();
-    return check_launch("kv_tree_umma");
+    if (int rc = check_launch("kv_tree_umma")) return rc;
+    launch_chained(kv_tree_merge_kernel<NR>, dim3((unsigned)(a.Hkv * p.groups * (NR / 8)), (unsigned)B), dim3(256), 0, st, a, B, p.groups, p.S, out,
+                   out_f32);
+    count_launch();
+    return check_launch("kv_tree_merge");
 }
 
 template <int U>
-int launch_tree_umma(const KvTreeArgs& a, const TreePlan& p, int B, cudaStream_t st) {
-    return p.rows == 16 ? launch_tree_umma_rows<U, 16>(a, p, B, st)
-         : p.rows == 32 ? launch_tree_umma_rows<U, 32>(a, p, B, st) : launch_tree_umma_rows<U, 64>(a, p, B, st);
+int launch_tree_umma(const KvTreeArgs& a, const TreePlan& p, int B, __nv_bfloat16* out, float* out_f32, cudaStream_t st) {
+    return p.rows == 16 ? launch_tree_umma_rows<U, 16>(a, p, B, out, out_f32, st)
+         : p.rows == 32 ? launch_tree_umma_rows<U, 32>(a, p, B, out, out_f32, st) : launch_tree_umma_rows<U, 64>(a, p, B, out, out_f32, st);
 }
 
 // Row groups x kv heads x sequences thread blocks of one key piece each; pieces until about three blocks per SM are there.
@@ -101,9 +96,11 @@ using namespace msaq;
 extern "C" size_t msaq_kv_tree_workspace(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk, int64_t D) {
     const DeviceScope device;
     if (!tree_sizes_ok(B, T, H, Hkv, Lk, D)) return 0;
-    int S = plan_tree_generic(B, T, H, Hkv, Lk).S;
-    if (D == 128) S = std::max(S, plan_tree_umma(B, T, H, Hkv, Lk).S);      // the same size for every format
-    const size_t bytes = (size_t)B * T * H * S * (D + 2) * sizeof(float);
+    size_t bytes = (size_t)B * T * H * plan_tree_generic(B, T, H, Hkv, Lk).S * (D + 2) * sizeof(float);
+    if (D == 128) {                                               // the same size for every format
+        const TreePlan p = plan_tree_umma(B, T, H, Hkv, Lk);
+        bytes = std::max(bytes, (size_t)2 * p.S * p.rows * KTU_PART * sizeof(float));
+    }
     return ((bytes + 255) & ~(size_t)255) + WS_CTL_BYTES;
 }
 
@@ -137,15 +134,20 @@ extern "C" int msaq_kv_tree_attention(const void* q, const int8_t* ks, const uin
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool tuned = umma_eligible(D, gs) &&
                        !((reinterpret_cast<uintptr_t>(ku) | reinterpret_cast<uintptr_t>(kh) | reinterpret_cast<uintptr_t>(vu) |
-                          reinterpret_cast<uintptr_t>(vh)) & 15);
+                          reinterpret_cast<uintptr_t>(vh)) & 15) &&
+                       !(reinterpret_cast<uintptr_t>(q) & 7);
     const TreePlan p = tuned ? plan_tree_umma(B, T, H, Hkv, Lk) : plan_tree_generic(B, T, H, Hkv, Lk);
     float* partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + WS_CTL_BYTES);
     const KvTreeArgs a{static_cast<const __nv_bfloat16*>(q), KvPlanes{ks, ku, kh}, KvPlanes{vs, vu, vh}, partial, lens, mask, mask_stride,
                        (int)T, (int)H, (int)Hkv, (int)Lk, (int)Lcap, (int)D, (int)NB, p.key_tile, p.S, qrot,
                        (float)(1.4426950408889634 / sqrt((double)D)), sticky_status(), option_wait_polls(), option_test_skip_stage(), f};
+    if (tuned) {
+        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(out);
+        return u == 4 ? launch_tree_umma<4>(a, p, (int)B, o, out_f32, st)
+             : u == 3 ? launch_tree_umma<3>(a, p, (int)B, o, out_f32, st) : launch_tree_umma<2>(a, p, (int)B, o, out_f32, st);
+    }
     int rc;
-    if (tuned) rc = u == 4 ? launch_tree_umma<4>(a, p, (int)B, st) : u == 3 ? launch_tree_umma<3>(a, p, (int)B, st) : launch_tree_umma<2>(a, p, (int)B, st);
-    else switch (D) {
+    switch (D) {
         case 32: rc = launch_tree_generic<1>(a, p, (int)B, st); break;
         case 64: rc = launch_tree_generic<2>(a, p, (int)B, st); break;
         case 128: rc = launch_tree_generic<4>(a, p, (int)B, st); break;

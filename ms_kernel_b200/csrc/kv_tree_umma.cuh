@@ -1,23 +1,28 @@
 // Tuned attention for a tree of drafted tokens over a packed cache: gs = 2, head_dim 128, any u, any Hq / Hkv, any capacity.
 //
-// A thread block takes up to 64 query rows (nodes x the heads of one kv head) against one piece of the keys, 128 at a time, with the
-// KEYS on the tensor cores' wide side:
+// A thread block (one per SM) takes up to 64 query rows (nodes x the heads of one kv head) against 128 keys at a time, with the KEYS on
+// the tensor cores' wide side:
 //     S^T[128 keys x rows] = K[128 x 128] . Q^T          P^T = 2^(S^T - m)          O^T[128 channels x rows] += V^T . P^T
-// so that the tensor and exponential work follow the number of rows, every thread of the softmax owns one key (its scale is one
-// register) and all warps have the same work whatever the number of rows.
-//   * Codes go from global memory to registers one tile ahead, thread = (key, two 32-blocks).  Keys become fp16 operands
-//     q 2^(e - e_max) relative to the largest exponent of THEIR row (exact down to 2^-24, 2^-31 of the row's largest value below) and
-//     go to tensor memory as operand A; the factor 2^e_max is applied to the scores.  The block's codes are 8-bit integers
-//     offset to bytes: a byte permute drops two of them into the mantissas of 1024.0, one fused multiply-add takes the offset out
-//     and the scale in.  Values become fp16 operands q 2^(e + 2) in shared memory, [key][channel] with the channel as the
-//     contiguous (M) dimension.
+// so that the tensor and exponential work follow the number of rows and every thread of the softmax owns one key (its scale is one
+// register).
+//   * Eight decode warps, thread = (key, two 32-blocks): codes go from global memory to registers one tile ahead.  Keys become fp16
+//     operands q 2^(e - e_max) relative to the largest exponent of THEIR row (exact down to 2^-24, 2^-31 of the row's largest
+//     value below) and go to tensor memory as operand A; the factor 2^e_max is applied to the scores.  A block's codes are
+//     8-bit integers offset to bytes: a byte permute drops two of them into the mantissas of 1024.0, one fused multiply-add
+//     takes the offset out and the scale in.  Values become fp16 operands q 2^(e + 2) in shared memory, [key][channel] with the
+//     channel as the contiguous (M) dimension.
 //   * A tile that holds a value block outside the exponents -26 .. 3 (2^-20 to 2^10 in magnitude) is done in bf16 instead, values and
 //     probabilities: the range of fp32 at eight digits, so that a row is not touched by the range of a key it does not see.
-//   * Queries are staged once, rotated in fp32, each row scaled by a power of two into fp16 (11 digits; the bf16 query has 8, its
-//     rotation more).  Probabilities are fp16 (11 digits), 2^7 above the running maximum's scale so that they reach down to 2^-31.
-//   * The maximum is lazy: a row's reference moves only when a score exceeds it by more than 2^8 -- one vote per tile -- and then
-//     the accumulators of those rows are rescaled in tensor memory.  Sums and accumulators are fp32.
-//   * Two thread blocks share an SM: one's conversions run under the other's MMAs and waits.
+//   * Queries are staged once per item, rotated in fp32, each row scaled by a power of two into fp16 (11 digits; the bf16 query
+//     has 8, its rotation more).  Probabilities are fp16 (11 digits), 2^7 above the reference's scale so that they reach down to 2^-31.
+//   * Eight softmax warps, thread = (key, half of the rows).  The maximum is lazy: a row's reference moves only when a score
+//     exceeds it by more than 2^8 -- one vote per tile of the four warps that hold the row -- and then the accumulators of the
+//     rows concerned are rescaled in tensor memory.  Sums and accumulators are fp32.
+//   * One warp issues the MMAs: S(i + 1) before P.V(i), so that both run under the decoding and the softmax.  Scores, key operands and
+//     probabilities have two buffers, values three; the roles meet on mbarriers only.
+//   * The tiles of all (sequence, kv head, row group) items form one line, cut into equal runs, one per thread block: ragged
+//     batches balance.  An item inside one run is finished there; one that is cut leaves partial results (acc, m, l), merged by a second
+//     kernel in the order of the runs.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -29,9 +34,11 @@
 
 namespace msaq {
 
-constexpr int KTU_THREADS = 256, KTU_KEYS = 128, KTU_ROWS = 64;
-constexpr int KTU_COL_O = 0, KTU_COL_S = 64, KTU_COL_K = 128, KTU_COLS = 256;      // tensor memory columns
-constexpr int KTU_V = 0, KTU_P = 32768, KTU_Q = KTU_P + 16384;                      // shared memory: values, probabilities, queries
+constexpr int KTU_WARPS = 8;                                                        // of each of the two working roles
+constexpr int KTU_THREADS = (2 * KTU_WARPS + 1) * 32, KTU_KEYS = 128, KTU_ROWS = 64, KTU_VBUFS = 3;
+constexpr int KTU_COL_O = 0, KTU_COL_S = 64, KTU_COL_K = 192, KTU_COLS = 512;       // tensor memory columns: O, two S, two K (320 used)
+constexpr int KTU_V = 0, KTU_P = KTU_VBUFS * 32768, KTU_Q = KTU_P + 2 * 16384;       // shared memory: values, probabilities, queries
+constexpr int KTU_PART = 132;                                                       // floats of a row's partial result: acc, m, l, padding
 __host__ __device__ constexpr int ktu_smem_bytes(int nr) { return KTU_Q + nr * 256 + 1024; }
 constexpr int KTU_V_BITS = 2;                                                       // values are held times 2^2
 constexpr float KTU_P_BITS = 7.0f, KTU_MOVE = 15.0f;                                // 2^7 at the reference, which moves at 2^15
@@ -63,7 +70,7 @@ __device__ __forceinline__ void ktu_st16(uint32_t taddr, const uint32_t (&r)[16]
         "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-// Eight accumulator columns of this warp's lanes; ktu_ld_wait() before they are used.
+// Eight accumulator columns of this warp's lanes.
 __device__ __forceinline__ void ktu_ld8(uint32_t taddr, float* v) {
     uint32_t r[8];
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -79,6 +86,47 @@ __device__ __forceinline__ void ktu_st8(uint32_t taddr, const float* v) {
                  "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])),
                  "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
                  : "memory");
+}
+// N accumulator columns (8, 16 or 32) in one access.
+template <int N> __device__ __forceinline__ void ktu_ld(uint32_t taddr, float (&v)[N]);
+template <> __device__ __forceinline__ void ktu_ld<8>(uint32_t taddr, float (&v)[8]) { ktu_ld8(taddr, v); }
+template <> __device__ __forceinline__ void ktu_ld<16>(uint32_t taddr, float (&v)[16]) { tmem_ld16(taddr, v); }
+template <> __device__ __forceinline__ void ktu_ld<32>(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+        "%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 __device__ __forceinline__ void ktu_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -110,46 +158,22 @@ template <> struct KtuRaw<4> { uint4 u; uint2 s; };
 template <> struct KtuRaw<3> { uint32_t u[5]; uint32_t s0, s1; };
 template <> struct KtuRaw<2> { uint2 u[3]; uint32_t s; };
 
-__device__ __forceinline__ uint4 ldg128(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+// The bytes of one block.
+__device__ __forceinline__ void ktu_load(KtuRaw<4>& r, const uint8_t* up, const uint8_t* sh) {
+    r.u = __ldcg(reinterpret_cast<const uint4*>(up));
+    r.s = __ldcg(reinterpret_cast<const uint2*>(sh));
 }
-__device__ __forceinline__ uint2 ldg64(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t ldg32(const void* p) {
-    uint32_t v;
-    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t ldg16(const void* p) {
-    uint16_t v;
-    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ int ldg_s8(const void* p) {
-    int v;
-    asm volatile("ld.global.s8 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-
-__device__ __forceinline__ void ktu_load(KtuRaw<4>& r, const KvPlanes& p, int64_t slot) {
-    r.u = ldg128(p.u + slot * 16);
-    r.s = ldg64(p.h + slot * 8);
-}
-__device__ __forceinline__ void ktu_load(KtuRaw<3>& r, const KvPlanes& p, int64_t slot) {
+__device__ __forceinline__ void ktu_load(KtuRaw<3>& r, const uint8_t* up, const uint8_t* sh) {
 #pragma unroll
-    for (int i = 0; i < 5; ++i) r.u[i] = ldg32(p.u + slot * 20 + 4 * i);
-    r.s0 = ldg16(p.h + slot * 6) | ldg16(p.h + slot * 6 + 2) << 16;
-    r.s1 = ldg16(p.h + slot * 6 + 4);
+    for (int k = 0; k < 5; ++k) r.u[k] = __ldca(reinterpret_cast<const uint32_t*>(up) + k);
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(sh);
+    r.s0 = __ldca(h) | (uint32_t)__ldca(h + 1) << 16;
+    r.s1 = __ldca(h + 2);
 }
-__device__ __forceinline__ void ktu_load(KtuRaw<2>& r, const KvPlanes& p, int64_t slot) {
+__device__ __forceinline__ void ktu_load(KtuRaw<2>& r, const uint8_t* up, const uint8_t* sh) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) r.u[i] = ldg64(p.u + slot * 24 + 8 * i);
-    r.s = ldg32(p.h + slot * 4);
+    for (int k = 0; k < 3; ++k) r.u[k] = __ldca(reinterpret_cast<const uint2*>(up) + k);
+    r.s = __ldcg(reinterpret_cast<const uint32_t*>(sh));
 }
 __device__ __forceinline__ void ktu_clear(KtuRaw<4>& r) { r.u = make_uint4(0u, 0u, 0u, 0u); r.s = make_uint2(0u, 0u); }
 __device__ __forceinline__ void ktu_clear(KtuRaw<3>& r) {
@@ -216,357 +240,736 @@ template <> __device__ __forceinline__ void ktu_codes<2>(const KtuRaw<2>& r, int
 template <int U> __host__ __device__ __forceinline__ int ktu_place(int e) { return U == 4 ? (e & ~7) | (e & 1) << 2 | (e >> 1 & 3) : e; }
 template <int U> __host__ __device__ __forceinline__ int ktu_element(int p) { return U == 4 ? (p & ~7) | (p >> 2 & 1) | (p & 3) << 1 : p; }
 
+// ---- the line of tiles -------------------------------------------------------------------------
+// Item (b, hk, group) has tiles_of(b) tiles; items in that order, sequences first.  Of the N tiles thread block c of C <= N takes
+// [c N / C, (c + 1) N / C).
+__device__ __forceinline__ int ktu_tiles(const KvTreeArgs& a, int b) { return (kt_len(a, b) + a.T + KTU_KEYS - 1) / KTU_KEYS; }
+__device__ __forceinline__ int64_t ktu_run(int64_t n, int c, int C) { return n / C * c + n % C * c / C; }        // c n / C without overflow
+// The thread block whose run holds tile g.
+__device__ __forceinline__ int ktu_owner(int64_t n, int64_t g, int C) {
+    int c = (int)min((int64_t)C - 1, (int64_t)((double)g * C / (double)n));
+    while (c > 0 && ktu_run(n, c, C) > g) --c;
+    while (c + 1 < C && ktu_run(n, c + 1, C) <= g) ++c;
+    return c;
+}
+
+// Sum of tiles_of over the sequences in front of `b` and over all, by the whole thread block of W warps; red: 2 W words of shared memory.
+template <int W>
+__device__ __forceinline__ void ktu_sums(const KvTreeArgs& a, int B, int b, long long* red, int64_t* before, int64_t* all) {
+    const int tid = threadIdx.x, warp = tid >> 5;
+    long long s = 0, t = 0;
+    for (int i = tid; i < B; i += W * 32) {
+        const int n = ktu_tiles(a, i);
+        t += n;
+        if (i < b) s += n;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if ((tid & 31) == 0) { red[warp] = s; red[W + warp] = t; }
+    __syncthreads();
+    s = t = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) { s += red[w]; t += red[W + w]; }
+    *before = s;
+    *all = t;
+    __syncthreads();
+}
+
+// A place on the line.
+struct KtuCursor {
+    int b, hk, grp, t;                                            // sequence, kv head, row group, tile
+    int len, tiles;                                               // of the sequence
+    __device__ __forceinline__ void sequence(const KvTreeArgs& a, int seq) {
+        b = seq;
+        len = kt_len(a, b);
+        tiles = (len + a.T + KTU_KEYS - 1) / KTU_KEYS;
+    }
+    __device__ __forceinline__ void next(const KvTreeArgs& a, int groups, int B) {
+        if (++t < tiles) return;
+        t = 0;
+        if (++grp < groups) return;
+        grp = 0;
+        if (++hk < a.Hkv) return;
+        hk = 0;
+        if (b + 1 < B) sequence(a, b + 1);
+    }
+};
+
+// Barrier of `threads` threads under number `id`, with a vote.
+__device__ __forceinline__ bool ktu_vote(int id, int threads, bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"((uint32_t)v), "r"(id), "r"(threads) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void ktu_bar(int id, int threads) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// Column sums over the 32 lanes: on return v[0] of lane c holds column c (N = 32), c % N below.
+template <int N> __device__ __forceinline__ void ktu_column_sums(float (&v)[N], int lane) {
+#pragma unroll
+    for (int s = N / 2; s >= 1; s >>= 1)
+#pragma unroll
+        for (int i = 0; i < s; ++i) {
+            const bool up = lane & s;
+            const float give = up ? v[i] : v[i + s];
+            v[i] = (up ? v[i + s] : v[i]) + __shfl_xor_sync(0xffffffffu, give, s);
+        }
+#pragma unroll
+    for (int s = N; s < 32; s <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], s);
+}
+
+struct __align__(16) KtuShared {
+    uint64_t kfull[4], vfull[KTU_VBUFS], sfull[2], pfull[2], qfull[4];        // written: keys, values, scores, probabilities, queries
+    uint64_t sempty[2], vempty[KTU_VBUFS], pempty[2], done;                   // read
+    uint32_t tmem;
+    int seq;
+    long long seq_tile, red[2 * (2 * KTU_WARPS + 1)];
+    volatile int abort;
+    int wide[4];                                                  // tile's values (and probabilities) are bf16
+    uint64_t mask[KT_MAX_T];
+    float qf[4][KTU_ROWS], qscale[4];                             // score factors 2^x of the query rows; of all rows where they are the same
+    int same[4], qtop[KTU_WARPS], qlow[KTU_WARPS];
+    float ck[4][KTU_KEYS];                                        // score factors of the keys
+    float4 ref4[KTU_ROWS / 4];                                    // per row 7 - m (+inf: nothing seen yet; NaN: not a number)
+    float f[KTU_ROWS];                                            // per row the score factor, where they differ
+    float m[KTU_ROWS], alpha[KTU_ROWS], part[4][KTU_ROWS];
+};
+
 template <int U, int NR>
-__global__ void __launch_bounds__(KTU_THREADS, 2)
-kv_tree_umma_kernel(const KvTreeArgs a) {
+__global__ void __launch_bounds__(KTU_THREADS, 1)
+kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32) {
     chain_wait();
     constexpr int NC = NR / 2;                                    // columns (query rows) of a thread in the softmax
     constexpr uint32_t OFFSET = 1024u + 128u + (1u << (U - 1));   // what the mantissa bytes stand above the codes
     extern __shared__ uint8_t ktu_smem_raw[];
-    __shared__ __align__(8) uint64_t bar_s, bar_pv, bar_done;
-    __shared__ uint32_t tmem_slot;
-    __shared__ uint64_t mask_s[KT_MAX_T];
-    __shared__ __align__(16) float2 ref[NR];                      // per row: score factor 2^x of the query row, 7 - m (+inf: nothing seen yet)
-    __shared__ float m_s[NR], alpha_s[NR], cmax[4][NR];
+    __shared__ KtuShared sh;
     const uint32_t sbase = (smem_u32(ktu_smem_raw) + 1023u) & ~1023u;
     uint8_t* const smem = ktu_smem_raw + (sbase - smem_u32(ktu_smem_raw));
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3, half = warp >> 2;
-    const bool issuer = __shfl_sync(0xffffffffu, warp, 0) == 0;    // the warp that issues the MMAs
-    const int key = quad * 32 + lane;                             // this thread's key of a tile; its blocks are 2 half, 2 half + 1
-    const int groups = gridDim.y / a.Hkv, hk = blockIdx.y / groups, grp = blockIdx.y % groups, b = blockIdx.z;
-    const int G = a.Hq / a.Hkv, R = a.T * G, r0 = grp * NR, rows = min(NR, R - r0);
-    const int len = kt_len(a, b);
-    const int j0 = blockIdx.x * a.key_tile, j1 = min(j0 + a.key_tile, len + a.T);
-    float* const out = a.partial + ((((int64_t)b * a.Hkv + hk) * R + r0) * a.S + blockIdx.x) * 130;
-    if (j1 <= j0) {                                               // no keys of this sequence in this piece
-        for (int r = tid; r < rows; r += KTU_THREADS) {
-            out[(int64_t)r * a.S * 130 + 128] = -INFINITY;
-            out[(int64_t)r * a.S * 130 + 129] = 0.0f;
-        }
-        return;
-    }
-    const int tiles = (j1 - j0 + KTU_KEYS - 1) / KTU_KEYS;
-    const int64_t krow = (((int64_t)b * a.Hkv + hk) * 4) * a.Lcap;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int role = warp / KTU_WARPS, quad = warp & 3, half = warp >> 2 & 1;      // role 0: decode, 1: softmax, 2: MMAs
+    const int key = quad * 32 + lane;                             // this thread's key of a tile
+    const int G = a.Hq / a.Hkv, R = a.T * G, per_seq = a.Hkv * groups;
 
-    KtuRaw<U> kraw[2], vraw[2];
-    int ke[4], ve[2];
-    auto load_k = [&](int it) {
-        const int j = j0 + it * KTU_KEYS + key;
-        const bool ok = j < j1;
+    // ---- this thread block's run of tiles, and where it begins ----
+    int64_t skip, total;
+    ktu_sums<2 * KTU_WARPS + 1>(a, B, 0, sh.red, &skip, &total);
+    total *= per_seq;
+    const int C = (int)min((int64_t)gridDim.x, total);            // no run is empty
+    if ((int)blockIdx.x >= C) return;
+    const int64_t g0 = ktu_run(total, blockIdx.x, C);
+    const int n_run = (int)(ktu_run(total, blockIdx.x + 1, C) - g0);
+    if (warp == 0) {                                              // sequences in steps of 32
+        long long base = 0;
+        for (int i0 = 0; i0 < B; i0 += 32) {
+            const long long n = i0 + lane < B ? (long long)ktu_tiles(a, i0 + lane) * per_seq : 0;
+            long long upto = n;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (ok) ktu_load(kraw[i], a.k, krow + (int64_t)(2 * half + i) * a.Lcap + j);
-            else ktu_clear(kraw[i]);
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            if (n && base + upto > g0 && base + upto - n <= g0) { sh.seq = i0 + lane; sh.seq_tile = base + upto - n; }
+            base += __shfl_sync(0xffffffffu, upto, 31);
+            if (base > g0) break;
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ke[i] = ok ? ldg_s8(a.k.s + krow + (int64_t)i * a.Lcap + j) : -127;
-    };
-    auto load_v = [&](int it) {
-        const int j = j0 + it * KTU_KEYS + key;
-        const bool ok = j < j1;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (ok) ktu_load(vraw[i], a.v, krow + (int64_t)(2 * half + i) * a.Lcap + j);
-            else ktu_clear(vraw[i]);
-            ve[i] = ok ? ldg_s8(a.v.s + krow + (int64_t)(2 * half + i) * a.Lcap + j) : 0;
-        }
-    };
-    load_k(0);
-    load_v(0);
-
-    if (tid == 0) {
-        mbar_init(smem_u32(&bar_s), 1);
-        mbar_init(smem_u32(&bar_pv), 1);
-        mbar_init(smem_u32(&bar_done), 1);
-        mbar_init_fence();
     }
-    if (warp == 0) {
-        tmem_alloc(smem_u32(&tmem_slot), KTU_COLS);
+    if (role == 2) {
+        tmem_alloc(smem_u32(&sh.tmem), KTU_COLS);
         tmem_relinquish();
     }
-    if (tid < a.T) mask_s[tid] = a.mask[b * a.mask_stride + tid];
-    // ---- queries: rotated, scaled by a power of two per row, fp16, K-major with 128-byte swizzle ----
-    for (int r = warp; r < NR; r += KTU_THREADS / 32) {
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < rows) {
-            const int row = r0 + r;
-            const __nv_bfloat16* qp = a.q + (((int64_t)b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + lane * 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __bfloat162float(qp[i]);
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&sh.kfull[i]), KTU_WARPS); mbar_init(smem_u32(&sh.qfull[i]), KTU_WARPS); }
+        for (int i = 0; i < KTU_VBUFS; ++i) { mbar_init(smem_u32(&sh.vfull[i]), KTU_WARPS); mbar_init(smem_u32(&sh.vempty[i]), 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh.sfull[i]), 1);
+            mbar_init(smem_u32(&sh.pfull[i]), KTU_WARPS);
+            mbar_init(smem_u32(&sh.sempty[i]), KTU_WARPS);
+            mbar_init(smem_u32(&sh.pempty[i]), 1);
         }
-        if (a.qrot) {
-            fwht_warp<4>(v, lane);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] *= 0.08838834764831845f;     // 1 / sqrt(128)
-        }
-        uint32_t ax = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ax = max(ax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        ax = __reduce_max_sync(0xffffffffu, ax);
-        const bool bad = ax >= 0x7F800000u;                       // an infinity or a NaN: the row is NaN, the others are not touched
-        const int E = max((int)(ax >> 23) - 127, -100);
-        const float up = __int_as_float((137 - E) << 23);          // largest element to [1024, 2048)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = ktu_place<U>(lane * 4 + i);
-            const __half h = __float2half_rn(bad ? 0.0f : v[i] * up);
-            *reinterpret_cast<__half*>(smem + KTU_Q + (p >> 6) * (NR * 128) + r * 128 + ((((p >> 3) & 7) ^ (r & 7)) << 4) + (p & 7) * 2) = h;
-        }
-        if (lane == 0) {
-            ref[r] = make_float2(bad ? __int_as_float(0x7FC00000) : exp2_int(E - 10), INFINITY);
-            m_s[r] = -INFINITY;
-        }
+        mbar_init(smem_u32(&sh.done), 1);
+        mbar_init_fence();
+        sh.abort = 0;
     }
-    fence_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tm = tmem_slot, tlane = tm + ((uint32_t)(quad * 32) << 16);
-    const uint32_t idesc_qk = ktu_idesc(NR, 0, 0);
-    const bool inject = a.skip_stage >= 0 && (blockIdx.x | blockIdx.y | blockIdx.z) == 0;
+    const uint32_t tm = sh.tmem, tlane = tm + ((uint32_t)(quad * 32) << 16);
+    KtuCursor cur;
+    cur.sequence(a, sh.seq);
+    {
+        const int item = (int)((g0 - sh.seq_tile) / cur.tiles);
+        cur.t = (int)(g0 - sh.seq_tile - (int64_t)item * cur.tiles);
+        cur.hk = item / groups;
+        cur.grp = item - cur.hk * groups;
+    }
+    const KtuCursor start = cur;
 
-    float l[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) l[i] = 0.0f;
-    bool ok = true;                                               // this thread's waits so far
+    // A bounded wait of the whole warp; false: it ran out, here or elsewhere.  A warp whose wait failed waits no more but goes on through
+    // the motions, since others of its role meet it at the named barriers; the outputs are marked in the end.
+    auto wait = [&](const uint64_t& bar, uint32_t phase) {
+        bool done = mbar_try_wait(smem_u32(&bar), phase & 1u);
+        for (uint32_t i = 0; !done && i < a.max_polls && !sh.abort; ++i) {
+            done = mbar_try_wait(smem_u32(&bar), phase & 1u);
+            if (i >= MBAR_FAST_POLLS) __nanosleep(128);
+        }
+        if (!done) sh.abort = 1;
+        return __all_sync(0xffffffffu, done) != 0;
+    };
+    auto arrive = [&](const uint64_t& bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar));
+    };
 
-#pragma unroll 1
-    for (int it = 0; it < tiles; ++it) {
-        // ---- keys to tensor memory ----
-        const int emax = max(max(ke[0], ke[1]), max(ke[2], ke[3]));
-        const float ck = a.sm_scale_log2 * exp2_int(emax);
+    if (role == 0) {
+        // ================================ decode ================================
+        KtuRaw<U> kraw[2], vraw[2];
+        int ke[4], ve[2];
+        constexpr int UB = 4 * (8 - U), SB = 2 * U;
+        const int64_t cap = a.Lcap;
+        // this thread's key of the next tile to load, in the planes of blocks 2 half (codes) and 0 (exponents of keys)
+        const uint8_t *ku, *kh, *vu, *vh;
+        const int8_t *ks, *vs;
+        int left;                                                 // keys of the sequence from this thread's one on
+        auto seek = [&](const KtuCursor& c) {
+            const int64_t s0 = ((int64_t)c.b * a.Hkv + c.hk) * 4 * cap + c.t * KTU_KEYS + key, s1 = s0 + 2 * half * cap;
+            ku = a.k.u + s1 * UB;
+            kh = a.k.h + s1 * SB;
+            ks = a.k.s + s0;
+            vu = a.v.u + s1 * UB;
+            vh = a.v.h + s1 * SB;
+            vs = a.v.s + s1;
+            left = c.len + a.T - c.t * KTU_KEYS - key;
+        };
+        auto load_k = [&]() {
+            if (left > 0) {
+                ktu_load(kraw[0], ku, kh);
+                ktu_load(kraw[1], ku + cap * UB, kh + cap * SB);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t sc = ktu_pow2_h2((half ? ke[2 + i] : ke[i]) - emax);
-            const uint32_t off = hmul2(sc, 0xE400E400u + (OFFSET - 1024u) * 0x00010001u);      // -OFFSET (fp16 counts in ones from 1024 to 2048)
-            uint32_t w[16];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t t[4];
-                ktu_codes<U>(kraw[i], c, t);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) w[4 * c + x] = hfma2(t[x], sc, off);
+                for (int i = 0; i < 4; ++i) ke[i] = __ldcg(ks + i * cap);
+            } else {
+                ktu_clear(kraw[0]);
+                ktu_clear(kraw[1]);
+                ke[0] = ke[1] = ke[2] = ke[3] = -127;
             }
-            ktu_st16(tlane + KTU_COL_K + half * 32 + i * 16, w);
-        }
-        if (it + 1 < tiles) load_k(it + 1);
-        // a value block outside the exponents that fp16 holds?
-        bool far = false;
+            ku += KTU_KEYS * UB;
+            kh += KTU_KEYS * SB;
+            ks += KTU_KEYS;
+        };
+        auto load_v = [&]() {
+            if (left > 0) {
+                ktu_load(vraw[0], vu, vh);
+                ktu_load(vraw[1], vu + cap * UB, vh + cap * SB);
+                ve[0] = __ldcg(vs);
+                ve[1] = __ldcg(vs + cap);
+            } else {
+                ktu_clear(vraw[0]);
+                ktu_clear(vraw[1]);
+                ve[0] = ve[1] = 0;
+            }
+            vu += KTU_KEYS * UB;
+            vh += KTU_KEYS * SB;
+            vs += KTU_KEYS;
+            left -= KTU_KEYS;
+        };
+        seek(cur);
+        load_k();
+        load_v();
+        int seg = -1, vbuf = 0;
+        uint32_t vphase = 0;
+        const uint32_t vrow = (half * 16384 + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;     // with the swizzle of chunk 0
+        bool ok = true;
+#pragma unroll 1
+        for (int j = 0; j < n_run; ++j) {
+            if (j == 0 || cur.t == 0) {
+                // ---- a new item: its queries, rotated, scaled by a power of two per row, fp16, K-major with 128-byte swizzle ----
+                ++seg;
+                if (j > 0) ok = ok && wait(sh.sfull[(j - 1) & 1], (uint32_t)(j - 1) >> 1);      // the last item's products have read theirs
+                const int hk = cur.hk, r0 = cur.grp * NR, rows = min(NR, R - r0);
+                constexpr int QR = NR / KTU_WARPS;                // rows of a warp
+                float v[QR][4];
+                int top = -128, low = 127;                        // exponents of the rows that are numbers and not zero
+                uint32_t bad = 0u;                                // rows with an infinity or a NaN: NaN, the others are not touched
+                int E[QR];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) far = far || ((ve[i] < -24 - KTU_V_BITS || ve[i] > 5 - KTU_V_BITS) && !ktu_zero(vraw[i]));
-        ktu_st_wait();
-        tc_fence_before();
-        const bool wide = __syncthreads_or(far);
-        if (issuer && elect_lane()) {
+                for (int k = 0; k < QR; ++k) {
+                    const int row = r0 + warp * QR + k;
+                    if (warp * QR + k < rows) {
+                        const uint2 raw = __ldcg(reinterpret_cast<const uint2*>(
+                            a.q + (((int64_t)cur.b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + lane * 4));
+                        v[k][0] = bf16_lo(raw.x); v[k][1] = bf16_hi(raw.x);
+                        v[k][2] = bf16_lo(raw.y); v[k][3] = bf16_hi(raw.y);
+                    } else {
+                        v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < QR; ++k) {
+                    if (a.qrot) {
+                        fwht_warp<4>(v[k], lane);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[k][i] *= 0.08838834764831845f;     // 1 / sqrt(128)
+                    }
+                    uint32_t ax = 0u;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ax = max(ax, __float_as_uint(v[k][i]) & 0x7FFFFFFFu);
+                    ax = __reduce_max_sync(0xffffffffu, ax);
+                    E[k] = max((int)(ax >> 23) - 127, -100);
+                    if (ax >= 0x7F800000u) bad |= 1u << k;
+                    else if (ax) { top = max(top, E[k]); low = min(low, E[k]); }
+                }
+                if (lane == 0) { sh.qtop[warp] = top; sh.qlow[warp] = low; }
+                ktu_bar(1, KTU_WARPS * 32);
+#pragma unroll
+                for (int w = 0; w < KTU_WARPS; ++w) { top = max(top, sh.qtop[w]); low = min(low, sh.qlow[w]); }
+                // largest element to [1024, 2048): of all rows where the smallest row still has its eleven digits then, else of each row
+                const bool same = low >= top - 12;
+#pragma unroll
+                for (int k = 0; k < QR; ++k) {
+                    const int r = warp * QR + k, e = max(same ? top : E[k], -100);
+                    const float up = __int_as_float((137 - e) << 23);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int p = ktu_place<U>(lane * 4 + i);
+                        const __half h = __float2half_rn(bad >> k & 1 ? 0.0f : v[k][i] * up);
+                        *reinterpret_cast<__half*>(smem + KTU_Q + (p >> 6) * (NR * 128) + r * 128 + ((((p >> 3) & 7) ^ (r & 7)) << 4) + (p & 7) * 2) = h;
+                    }
+                    if (lane == 0) sh.qf[seg & 3][r] = bad >> k & 1 ? __int_as_float(0x7FC00000) : exp2_int(e - 10);
+                }
+                if (tid == 0) { sh.same[seg & 3] = same; sh.qscale[seg & 3] = exp2_int(max(top, -100) - 10); }
+                fence_async_smem();
+                arrive(sh.qfull[seg & 3]);
+            }
+            // ---- keys to tensor memory, once the product before the last has read the buffer ----
+            if (j > 1) ok = ok && wait(sh.sfull[j & 1], (uint32_t)(j - 2) >> 1);
             tc_fence_after();
-            const uint32_t bhi = ktu_desc_hi(1024);
+            const int emax = max(max(ke[0], ke[1]), max(ke[2], ke[3]));
+            if (half == 0) sh.ck[j & 3][key] = a.sm_scale_log2 * exp2_int(emax);
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-                ktu_mma_ts(tm + KTU_COL_S, tm + KTU_COL_K + 8 * s, umma_desc_lo(sbase + KTU_Q + (s >> 2) * (NR * 128) + (s & 3) * 32, 16), bhi,
-                           idesc_qk, s > 0);
-            if (!(inject && it == a.skip_stage)) tc_commit(smem_u32(&bar_s));
-        }
-        // ---- values to shared memory, once the last tile's product has read them ----
-        if (it > 0) ok = ok && mbar_wait_bounded(smem_u32(&bar_pv), (uint32_t)(it - 1) & 1u, a.max_polls);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t row = sbase + KTU_V + half * 16384 + (key >> 3) * 1024 + (key & 7) * 128;
-            if (!wide) {
-                const uint32_t sc = ktu_pow2_h2(ktu_zero(vraw[i]) ? -100 : ve[i] + KTU_V_BITS);
-                const uint32_t off = hmul2(sc, 0xE400E400u + (OFFSET - 1024u) * 0x00010001u);
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t sc = ktu_pow2_h2((half ? ke[2 + i] : ke[i]) - emax);
+                const uint32_t off = hmul2(sc, 0xE400E400u + (OFFSET - 1024u) * 0x00010001u);  // -OFFSET (fp16 counts in ones from 1024 to 2048)
+                uint32_t w[16];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t t[4];
-                    ktu_codes<U>(vraw[i], c, t);
-                    sts128(row + (((i * 4 + c) ^ (key & 7)) << 4), hfma2(t[0], sc, off), hfma2(t[1], sc, off), hfma2(t[2], sc, off),
-                           hfma2(t[3], sc, off));
+                    ktu_codes<U>(kraw[i], c, t);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) w[4 * c + x] = hfma2(t[x], sc, off);
+                }
+                ktu_st16(tlane + KTU_COL_K + (j & 1) * 64 + half * 32 + i * 16, w);
+            }
+            cur.next(a, groups, B);
+            if (j + 1 < n_run) {
+                if (cur.t == 0) seek(cur);
+                load_k();
+            }
+            ktu_st_wait();
+            tc_fence_before();
+            arrive(sh.kfull[j & 3]);
+            // ---- values to shared memory, once the buffer's last product has read them; a block outside the exponents that fp16 holds? ----
+            bool far = (unsigned)(ve[0] + 24 + KTU_V_BITS) > 29u || (unsigned)(ve[1] + 24 + KTU_V_BITS) > 29u;
+            if (far) far = ((unsigned)(ve[0] + 24 + KTU_V_BITS) > 29u && !ktu_zero(vraw[0])) || ((unsigned)(ve[1] + 24 + KTU_V_BITS) > 29u && !ktu_zero(vraw[1]));
+            const bool wide = ktu_vote(1, KTU_WARPS * 32, far);
+            if (tid == 0) sh.wide[j & 3] = wide;
+            if (j >= KTU_VBUFS) ok = ok && wait(sh.vempty[vbuf], vphase ^ 1u);
+            const uint32_t row = sbase + KTU_V + vbuf * 32768 + vrow;
+            if (!wide) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t sc = ktu_pow2_h2(min(max(ve[i], -24 - KTU_V_BITS), 5 - KTU_V_BITS) + KTU_V_BITS);   // (out of range: zeros)
+                    const uint32_t off = hmul2(sc, 0xE400E400u + (OFFSET - 1024u) * 0x00010001u);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t t[4];
+                        ktu_codes<U>(vraw[i], c, t);
+                        sts128(row ^ (i * 4 + c) << 4, hfma2(t[0], sc, off), hfma2(t[1], sc, off), hfma2(t[2], sc, off),
+                               hfma2(t[3], sc, off));
+                    }
                 }
             } else {
-                const float sc = exp2_int(max(-126, min(116, ve[i] + KTU_V_BITS)));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t t[4];
-                    ktu_codes<U>(vraw[i], c, t);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float f0 = (float)((int)(t[x] & 0xFFu) - (int)(OFFSET - 1024u)) * sc;
-                        const float f1 = (float)((int)(t[x] >> 16 & 0xFFu) - (int)(OFFSET - 1024u)) * sc;
-                        t[x] = prmt(__float_as_uint(f0), __float_as_uint(f1), 0x7632u);      // eight digits: exact
-                    }
-                    sts128(row + (((i * 4 + c) ^ (key & 7)) << 4), t[0], t[1], t[2], t[3]);
-                }
-            }
-        }
-        if (it + 1 < tiles) load_v(it + 1);
-        // ---- scores ----
-        ok = ok && mbar_wait_bounded(smem_u32(&bar_s), (uint32_t)it & 1u, a.max_polls);
-        tc_fence_after();
-        const int jb = j0 + it * KTU_KEYS;
-        const bool tail = jb + KTU_KEYS > len;
-        uint32_t vis = 0xFFFFFFFFu;                               // which of this thread's rows attend its key
-        if (tail) {
-            const int j = jb + key - len;                         // below 0: in front of the tree
-            if (j >= 0) {
-                vis = 0u;
-                if (j < a.T)
-                    for (int c = 0; c < NC; ++c) {
-                        const int node = (r0 + half * NC + c) / G;
-                        if (node < a.T && (mask_s[node] >> j & 1)) vis |= 1u << c;
-                    }
-            }
-        }
-        float x[NC];
-#pragma unroll
-        for (int c = 0; c < NC; c += 8) {
-            ktu_ld8(tlane + KTU_COL_S + half * NC + c, &x[c]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float2 rf = ref[half * NC + c + k];
-                x[c + k] = fmaf(x[c + k] * ck, rf.x, rf.y);
-            }
-        }
-        if (tail)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-                if (!(vis >> c & 1)) x[c] = -INFINITY;
-        float top = x[0];
-#pragma unroll
-        for (int c = 1; c < NC; ++c) top = fmaxf(top, x[c]);
-        const bool move = it == 0 || top > KTU_MOVE;
-        if (__syncthreads_or(move)) {
-            // ---- references move: rows whose maximum of this tile is beyond theirs ----
 #pragma unroll 1
-            for (int c = 0; c < NC; c += 8) {
-                float s[8];
-                ktu_ld8(tlane + KTU_COL_S + half * NC + c, s);
+                for (int i = 0; i < 2; ++i) {
+                    const float sc = exp2_int(max(-126, min(116, (i ? ve[1] : ve[0]) + KTU_V_BITS)));
+                    const KtuRaw<U> raw = i ? vraw[1] : vraw[0];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    float t = s[k] * ck * ref[half * NC + c + k].x;
-                    if (!(vis >> (c + k) & 1) || t != t) t = -INFINITY;
-                    const int o = __float_as_int(t);                      // in the order of whole numbers
-                    const int mx = __reduce_max_sync(0xffffffffu, o ^ (o >> 31 & 0x7FFFFFFF));
-                    if (lane == 0) cmax[quad][half * NC + c + k] = __int_as_float(mx ^ (mx >> 31 & 0x7FFFFFFF));
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t t[4];
+                        ktu_codes<U>(raw, c, t);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float f0 = (float)((int)(t[x] & 0xFFu) - (int)(OFFSET - 1024u)) * sc;
+                            const float f1 = (float)((int)(t[x] >> 16 & 0xFFu) - (int)(OFFSET - 1024u)) * sc;
+                            t[x] = prmt(__float_as_uint(f0), __float_as_uint(f1), 0x7632u);      // eight digits: exact
+                        }
+                        sts128(row ^ (i * 4 + c) << 4, t[0], t[1], t[2], t[3]);
+                    }
                 }
             }
-            if (it > 0) ok = ok && mbar_wait_bounded(smem_u32(&bar_pv), (uint32_t)(it - 1) & 1u, a.max_polls);
-            __syncthreads();
-            if (tid < NR) {
-                const float mx = fmaxf(fmaxf(cmax[0][tid], cmax[1][tid]), fmaxf(cmax[2][tid], cmax[3][tid]));
-                float al = 1.0f;
-                const float m = m_s[tid];
-                if (mx > -INFINITY && (m == -INFINITY || mx - m > KTU_MOVE - KTU_P_BITS)) {
-                    al = m == -INFINITY ? 0.0f : ktu_exp2(m - mx);
-                    m_s[tid] = mx;
-                    ref[tid].y = KTU_P_BITS - mx;
+            if (j + 1 < n_run) load_v();
+            fence_async_smem();
+            arrive(sh.vfull[vbuf]);
+            if (++vbuf == KTU_VBUFS) { vbuf = 0; vphase ^= 1u; }
+        }
+    } else if (role == 1) {
+        // ================================ softmax ================================
+        const uint32_t prow = (sbase + KTU_P + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;
+        const int stid = tid - KTU_WARPS * 32, htid = stid & 127;             // thread of the role, of its half
+        int seg = -1, n_seg = 0, vbuf = 0;
+        uint32_t vphase = 0;
+        bool ok = true;
+        bool same = true;                                         // the item's query rows have one score factor
+        float qscale = 1.0f;
+        uint64_t l[NC / 2];                                       // sums of pairs of rows over this thread's keys
+#pragma unroll 1
+        for (int j = 0; j < n_run; ++j) {
+            const int r0 = cur.grp * NR;
+            if (j == 0 || cur.t == 0) {
+                ++seg;
+                n_seg = 0;
+                ok = ok && wait(sh.qfull[seg & 3], (uint32_t)seg >> 2);
+                ktu_bar(2, KTU_WARPS * 32);                       // the last item's masks and references are read
+                if (stid < a.T) sh.mask[stid] = a.mask[cur.b * a.mask_stride + stid];
+                if (stid < NR) {
+                    const float f = sh.qf[seg & 3][stid];
+                    sh.f[stid] = f;
+                    reinterpret_cast<float*>(sh.ref4)[stid] = f != f ? f : INFINITY;
+                    sh.m[stid] = -INFINITY;
                 }
-                alpha_s[tid] = al;
+                same = sh.same[seg & 3] != 0;
+                qscale = sh.qscale[seg & 3];
+                ktu_bar(2, KTU_WARPS * 32);
+#pragma unroll
+                for (int c = 0; c < NC / 2; ++c) l[c] = 0ull;
             }
-            __syncthreads();
+            const int jb = cur.t * KTU_KEYS;
+            const bool tail = jb + KTU_KEYS > cur.len;            // the tile has nodes of the tree
+            ok = ok && wait(sh.kfull[j & 3], (uint32_t)j >> 2);
+            const float ck = same ? sh.ck[j & 3][key] * qscale : sh.ck[j & 3][key];
+            uint32_t vis = 0xFFFFFFFFu;                           // which of this thread's rows attend its key
+            if (tail) {
+                const int k = jb + key - cur.len;                 // below 0: in front of the tree
+                if (k >= 0) {
+                    vis = 0u;
+                    if (k < a.T)
+                        for (int c = 0; c < NC; ++c) {
+                            const int node = (r0 + half * NC + c) / G;
+                            if (node < a.T && (sh.mask[node] >> k & 1)) vis |= 1u << c;
+                        }
+                }
+            }
+            ok = ok && wait(sh.sfull[j & 1], (uint32_t)j >> 1);
             tc_fence_after();
+            const uint32_t scol = tlane + KTU_COL_S + (j & 1) * 64 + half * NC;
+            float x[NC];
+            auto scores = [&]() {                                 // exponents of this tile's probabilities on the present references
+                ktu_ld<NC>(scol, x);
+                const uint64_t ck2 = pack2(ck, ck);
+                if (!same)
 #pragma unroll
-            for (int c = 0; c < NC; c += 8) {
-                float o[8];
-                if (it > 0) {
+                    for (int c = 0; c < NC; ++c) x[c] *= sh.f[half * NC + c];
+#pragma unroll
+                for (int c = 0; c < NC; c += 4) {
+                    const float4 rf = sh.ref4[(half * NC + c) / 4];
+                    unpack2(fma2(pack2(x[c], x[c + 1]), ck2, pack2(rf.x, rf.y)), x[c], x[c + 1]);
+                    unpack2(fma2(pack2(x[c + 2], x[c + 3]), ck2, pack2(rf.z, rf.w)), x[c + 2], x[c + 3]);
+                }
+                if (tail)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        if (!(vis >> c & 1)) x[c] = -INFINITY;
+            };
+            scores();
+            float top = x[0], top1 = x[1];
+#pragma unroll
+            for (int c = 2; c < NC; c += 2) {
+                top = fmaxf(top, x[c]);
+                top1 = fmaxf(top1, x[c + 1]);
+            }
+            top = fmaxf(top, top1);
+            // the product before the last has read this tile's buffer of the probabilities
+            if (j > 1) ok = ok && wait(sh.pempty[j & 1], (uint32_t)(j - 2) >> 1);
+            if (ktu_vote(3 + half, KTU_WARPS * 16, n_seg == 0 || top > KTU_MOVE)) {
+                // ---- references move: rows of this half whose maximum of this tile is beyond theirs ----
+                if (n_seg > 0) ok = ok && wait(sh.pempty[(j - 1) & 1], (uint32_t)(j - 1) >> 1);  // the accumulators are at rest
+#pragma unroll 1
+                for (int c = 0; c < NC; c += 8) {
+                    float s[8];
+                    ktu_ld8(scol + c, s);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = half * NC + c + k;
+                        float t = s[k] * ck * (same ? 1.0f : sh.f[r]);
+                        if (!(vis >> (c + k) & 1) || t != t) t = -INFINITY;
+                        const int o = __float_as_int(t);                      // in the order of whole numbers
+                        const int mx = __reduce_max_sync(0xffffffffu, o ^ (o >> 31 & 0x7FFFFFFF));
+                        if (lane == 0) sh.part[quad][r] = __int_as_float(mx ^ (mx >> 31 & 0x7FFFFFFF));
+                    }
+                }
+                ktu_bar(3 + half, KTU_WARPS * 16);
+                if (htid < NC) {
+                    const int r = half * NC + htid;
+                    const float mx = fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), m = sh.m[r];
+                    float al = 1.0f;
+                    float* const rf = reinterpret_cast<float*>(sh.ref4) + r;
+                    if (*rf == *rf && mx > -INFINITY && (m == -INFINITY || mx - m > KTU_MOVE - KTU_P_BITS)) {
+                        al = m == -INFINITY ? 0.0f : ktu_exp2(m - mx);
+                        sh.m[r] = mx;
+                        *rf = KTU_P_BITS - mx;
+                    }
+                    sh.alpha[r] = al;
+                }
+                ktu_bar(3 + half, KTU_WARPS * 16);
+                tc_fence_after();
+                if (n_seg > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < NC; c += 8) {
+                        float o[8];
+                        ktu_ld8(tlane + KTU_COL_O + half * NC + c, o);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float al = sh.alpha[half * NC + c + k];
+                            o[k] = al == 0.0f ? 0.0f : o[k] * al;
+                        }
+                        ktu_st8(tlane + KTU_COL_O + half * NC + c, o);
+                    }
+#pragma unroll
+                    for (int c = 0; c < NC; c += 2) {
+                        const float al0 = sh.alpha[half * NC + c], al1 = sh.alpha[half * NC + c + 1];
+                        float l0, l1;
+                        unpack2(l[c / 2], l0, l1);
+                        l[c / 2] = pack2(al0 == 0.0f ? 0.0f : l0 * al0, al1 == 0.0f ? 0.0f : l1 * al1);
+                    }
+                    ktu_st_wait();
+                }
+                scores();
+            }
+            tc_fence_before();
+            arrive(sh.sempty[j & 1]);
+            // ---- probabilities to shared memory, in the type of the tile's values ----
+            ok = ok && wait(sh.vfull[vbuf], vphase);
+            const bool wide = sh.wide[j & 3] != 0;
+            if (++vbuf == KTU_VBUFS) { vbuf = 0; vphase ^= 1u; }
+            const uint32_t pr = prow + (j & 1) * 16384;
+            auto store_p = [&](auto bf16) {
+#pragma unroll
+                for (int c = 0; c < NC; c += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        const float p0 = ktu_exp2(x[c + k]), p1 = ktu_exp2(x[c + k + 1]);
+                        l[(c + k) / 2] = add2(l[(c + k) / 2], pack2(p0, p1));
+                        if constexpr (!decltype(bf16)::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
+                        else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
+                    }
+                    sts128(pr ^ (half * (NC / 8) + c / 8) << 4, w[0], w[1], w[2], w[3]);
+                }
+            };
+            if (wide) store_p(std::true_type{});
+            else store_p(std::false_type{});
+            fence_async_smem();
+            tc_fence_before();
+            arrive(sh.pfull[j & 1]);
+            ++n_seg;
+
+            if (cur.t == cur.tiles - 1 || j == n_run - 1) {
+                // ---- the segment's result ----
+                const bool whole = n_seg == cur.tiles;            // finished here; else partial result 2 c (not the item's first) or 2 c + 1
+                float* const part = a.partial + ((int64_t)2 * blockIdx.x + (cur.t == n_seg - 1 ? 1 : 0)) * NR * KTU_PART;
+                const int rows = min(NR, R - r0), hk = cur.hk;
+                {
+                    float v[NC];
+#pragma unroll
+                    for (int c = 0; c < NC; c += 2) unpack2(l[c / 2], v[c], v[c + 1]);
+                    ktu_column_sums<NC>(v, lane);
+                    if (lane < NC) sh.part[quad][half * NC + lane] = v[0];
+                }
+                ktu_bar(3 + half, KTU_WARPS * 16);
+                if (htid < NC) {
+                    const int r = half * NC + htid;
+                    const float s = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
+                    sh.alpha[r] = s == 0.0f ? 0.0f : 1.0f / s;
+                    if (!whole && r < rows) {
+                        part[r * KTU_PART + 128] = sh.m[r];
+                        part[r * KTU_PART + 129] = s;
+                    }
+                }
+                ktu_bar(3 + half, KTU_WARPS * 16);
+                ok = ok && wait(sh.pempty[j & 1], (uint32_t)j >> 1);
+                tc_fence_after();
+                const int ch = ktu_element<U>(key);                           // accumulator lane = operand place of the channel
+#pragma unroll 1
+                for (int c = 0; c < NC; c += 8) {
+                    float o[8];
                     ktu_ld8(tlane + KTU_COL_O + half * NC + c, o);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const float al = alpha_s[half * NC + c + k];
-                        o[k] = al == 0.0f ? 0.0f : o[k] * al;
+                        const int r = half * NC + c + k;
+                        if (r >= rows) continue;
+                        if (whole) {
+                            const int row = r0 + r;
+                            const float f = sh.alpha[r], v = f == 0.0f ? 0.0f : o[k] * (1.0f / (1 << KTU_V_BITS)) * f;
+                            const int64_t at = (((int64_t)cur.b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + ch;
+                            out[at] = __float2bfloat16_rn(v);
+                            if (out_f32) out_f32[at] = v;
+                        } else {
+                            part[r * KTU_PART + ch] = o[k] * (1.0f / (1 << KTU_V_BITS));
+                        }
                     }
-                    ktu_st8(tlane + KTU_COL_O + half * NC + c, o);
                 }
-                ktu_ld8(tlane + KTU_COL_S + half * NC + c, &x[c]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float al = alpha_s[half * NC + c + k];
-                    l[c + k] = al == 0.0f ? 0.0f : l[c + k] * al;
-                    const float2 rf = ref[half * NC + c + k];
-                    x[c + k] = fmaf(x[c + k] * ck, rf.x, rf.y);
-                    if (!(vis >> (c + k) & 1)) x[c + k] = -INFINITY;
-                }
+                tc_fence_before();
             }
-            ktu_st_wait();
-        }
-        // ---- probabilities to shared memory ----
-        auto store_p = [&](auto bf16) {
-#pragma unroll
-            for (int c = 0; c < NC; c += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int k = 0; k < 8; k += 2) {
-                    const float p0 = ktu_exp2(x[c + k]), p1 = ktu_exp2(x[c + k + 1]);
-                    l[c + k] += p0;
-                    l[c + k + 1] += p1;
-                    if constexpr (!decltype(bf16)::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
-                    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
-                }
-                sts128(sbase + KTU_P + (key >> 3) * 1024 + (key & 7) * 128 + (((half * (NC / 8) + c / 8) ^ (key & 7)) << 4), w[0], w[1], w[2], w[3]);
-            }
-        };
-        if (wide) store_p(std::true_type{});
-        else store_p(std::false_type{});
-        fence_async_smem();
-        tc_fence_before();
-        const bool give_up = __syncthreads_or(!ok);
-        if (give_up) {
-            ok = false;
-            break;
-        }
-        if (issuer && elect_lane()) {
-            tc_fence_after();
-            const uint32_t hi = ktu_desc_hi(1024), id = ktu_idesc(NR, wide ? 1u : 0u, 1u);
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-                ktu_mma_ss(tm + KTU_COL_O, umma_desc_lo(sbase + KTU_V + s * 2048, 16384), hi, umma_desc_lo(sbase + KTU_P + s * 2048, 8192), hi, id,
-                           it > 0 || s > 0);
-            tc_commit(smem_u32(&bar_pv));
-        }
-    }
-
-    // ---- the piece's result ----
-    if (ok) ok = mbar_wait_bounded(smem_u32(&bar_pv), (uint32_t)(tiles - 1) & 1u, a.max_polls);
-    const bool done = !__syncthreads_or(!ok);
-    if (done) {
-        tc_fence_after();
-        float* const ls = reinterpret_cast<float*>(smem + KTU_V);         // [NR][132] sums of the 128 keys' threads
-#pragma unroll
-        for (int c = 0; c < NC; ++c) ls[(half * NC + c) * 132 + key] = l[c];
-        const int ch = ktu_element<U>(key);                               // accumulator lane = operand place of the channel
-#pragma unroll 1
-        for (int c = 0; c < NC; c += 8) {
-            float o[8];
-            ktu_ld8(tlane + KTU_COL_O + half * NC + c, o);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int r = half * NC + c + k;
-                if (r < rows) out[(int64_t)r * a.S * 130 + ch] = o[k] * (1.0f / (1 << KTU_V_BITS));
-            }
-        }
-        tc_fence_before();
-        __syncthreads();
-        for (int r = warp; r < rows; r += KTU_THREADS / 32) {
-            float s = (ls[r * 132 + lane] + ls[r * 132 + 32 + lane]) + (ls[r * 132 + 64 + lane] + ls[r * 132 + 96 + lane]);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (lane == 0) {
-                out[(int64_t)r * a.S * 130 + 128] = m_s[r];
-                out[(int64_t)r * a.S * 130 + 129] = s;
-            }
+            cur.next(a, groups, B);
         }
     } else {
-        for (int r = tid; r < rows; r += KTU_THREADS) out[(int64_t)r * a.S * 130 + 128] = __int_as_float(0x7FC00000);
-        if (tid == 0) {
-            report_wait_failure(a.sticky, WAIT_FAIL_KV_DECODE);
-            tc_commit(smem_u32(&bar_done));                               // nothing may still write tensor memory when it is returned
-            mbar_wait_bounded(smem_u32(&bar_done), 0);
+        // ================================ MMAs ================================
+        const uint32_t idesc_qk = ktu_idesc(NR, 0, 0), hi = ktu_desc_hi(1024);
+        int seg = -1, vbuf = 0;
+        uint32_t vphase = 0;
+        KtuCursor ahead = cur;                                    // of the scores' product, one tile in front
+        auto issue_qk = [&](int j) {
+            if (j == 0 || ahead.t == 0) {
+                ++seg;
+                if (!wait(sh.qfull[seg & 3], (uint32_t)seg >> 2)) return false;
+            }
+            if (!wait(sh.kfull[j & 3], (uint32_t)j >> 2)) return false;
+            if (j > 1 && !wait(sh.sempty[j & 1], (uint32_t)(j - 2) >> 1)) return false;
+            tc_fence_after();
+            if (elect_lane()) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    ktu_mma_ts(tm + KTU_COL_S + (j & 1) * 64, tm + KTU_COL_K + (j & 1) * 64 + 8 * s,
+                               umma_desc_lo(sbase + KTU_Q + (s >> 2) * (NR * 128) + (s & 3) * 32, 16), hi, idesc_qk, s > 0);
+                if (!(a.skip_stage == j && blockIdx.x == 0)) tc_commit(smem_u32(&sh.sfull[j & 1]));
+            }
+            __syncwarp();
+            ahead.next(a, groups, B);
+            return true;
+        };
+        bool first = true;                                        // the next product begins a segment: it overwrites the accumulators
+        if (issue_qk(0))
+#pragma unroll 1
+            for (int j = 0; j < n_run; ++j) {
+                if (j + 1 < n_run && !issue_qk(j + 1)) break;
+                if (!wait(sh.vfull[vbuf], vphase) || !wait(sh.pfull[j & 1], (uint32_t)j >> 1)) break;
+                tc_fence_after();
+                const uint32_t id = ktu_idesc(NR, sh.wide[j & 3] ? 1u : 0u, 1u);
+                if (elect_lane()) {
+#pragma unroll
+                    for (int s = 0; s < 8; ++s)
+                        ktu_mma_ss(tm + KTU_COL_O, umma_desc_lo(sbase + KTU_V + vbuf * 32768 + s * 2048, 16384), hi,
+                                   umma_desc_lo(sbase + KTU_P + (j & 1) * 16384 + s * 2048, 8192), hi, id, !first || s > 0);
+                    tc_commit(smem_u32(&sh.vempty[vbuf]));
+                    tc_commit(smem_u32(&sh.pempty[j & 1]));
+                }
+                __syncwarp();
+                if (++vbuf == KTU_VBUFS) { vbuf = 0; vphase ^= 1u; }
+                first = cur.t == cur.tiles - 1;
+                cur.next(a, groups, B);
+            }
+        // nothing may still write tensor memory when it is returned
+        if (elect_lane()) {
+            tc_commit(smem_u32(&sh.done));
+            mbar_wait_bounded(smem_u32(&sh.done), 0);
         }
-        tc_fence_before();
+        __syncwarp();
     }
+
+    tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
-        tc_fence_after();
-        tmem_dealloc(tm, KTU_COLS);
+    tc_fence_after();
+    if (role == 2) tmem_dealloc(tm, KTU_COLS);
+    if (sh.abort) {
+        // a wait gave up: everything of this run is marked
+        if (tid == 0) report_wait_failure(a.sticky, WAIT_FAIL_KV_DECODE);
+        cur = start;
+        for (int j = 0, n_seg = 0; j < n_run; ++j) {
+            ++n_seg;
+            if (cur.t == cur.tiles - 1 || j == n_run - 1) {
+                const int r0 = cur.grp * NR, rows = min(NR, R - r0), hk = cur.hk;
+                float* const part = a.partial + ((int64_t)2 * blockIdx.x + (cur.t == n_seg - 1 ? 1 : 0)) * NR * KTU_PART;
+                for (int i = tid; i < rows * 128; i += KTU_THREADS) {
+                    const int row = r0 + (i >> 7);
+                    const int64_t o = (((int64_t)cur.b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + (i & 127);
+                    if (n_seg == cur.tiles) {
+                        out[o] = __float2bfloat16_rn(__int_as_float(0x7FC00000));
+                        if (out_f32) out_f32[o] = __int_as_float(0x7FC00000);
+                    } else if ((i & 127) == 0) {
+                        part[(i >> 7) * KTU_PART + 128] = __int_as_float(0x7FC00000);
+                    }
+                }
+                n_seg = 0;
+            }
+            cur.next(a, groups, B);
+        }
+    }
+}
+
+// Merge of the items that were cut: a warp per row, the runs' results in their order.  Run c left an item's first part in slot 2 c + 1 and
+// any other in slot 2 c.  A NaN in m marks a run whose wait gave up.
+template <int NR>
+__global__ void __launch_bounds__(256)
+kv_tree_merge_kernel(const KvTreeArgs a, int B, int groups, int blocks, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32) {
+    chain_release();
+    chain_wait();
+    __shared__ long long red[16];
+    const int per_seq = a.Hkv * groups, G = a.Hq / a.Hkv, R = a.T * G;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.y, item = blockIdx.x / (NR / 8), r = blockIdx.x % (NR / 8) * 8 + warp;
+    const int hk = item / groups, row = item % groups * NR + r;
+    int64_t before, total;
+    ktu_sums<8>(a, B, b, red, &before, &total);
+    total *= per_seq;
+    const int C = (int)min((int64_t)blocks, total), tiles = ktu_tiles(a, b);
+    const int64_t g = before * per_seq + (int64_t)item * tiles;
+    const int first = ktu_owner(total, g, C), last = ktu_owner(total, g + tiles - 1, C);
+    if (first == last || row >= R) return;
+    const int n = last - first + 1;
+    auto slot = [&](int i) { return a.partial + (((int64_t)2 * (first + i) + (i == 0 ? 1 : 0)) * NR + r) * KTU_PART; };
+    float mg = -INFINITY;
+    bool bad = false;
+    for (int i = lane; i < n; i += 32) {
+        const float m = slot(i)[128];
+        bad = bad || m != m;
+        mg = fmaxf(mg, m);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mg = fmaxf(mg, __shfl_xor_sync(0xffffffffu, mg, o));
+    bad = __any_sync(0xffffffffu, bad);
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, den = 0.0f;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+        float4 v[8];
+        float m[8], l[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (i0 + k >= n) continue;
+            const float* p = slot(i0 + k);
+            v[k] = *reinterpret_cast<const float4*>(p + 4 * lane);
+            m[k] = p[128];
+            l[k] = p[129];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (i0 + k >= n || (m[k] == -INFINITY && l[k] == 0.0f)) continue;     // a part of which the row attends nothing
+            const float w = exp2f(m[k] - mg);
+            acc[0] = fmaf(v[k].x, w, acc[0]);
+            acc[1] = fmaf(v[k].y, w, acc[1]);
+            acc[2] = fmaf(v[k].z, w, acc[2]);
+            acc[3] = fmaf(v[k].w, w, acc[3]);
+            den = fmaf(l[k], w, den);
+        }
+    }
+    const float f = den == 0.0f ? 0.0f : 1.0f / den;
+    const int64_t o = (((int64_t)b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + 4 * lane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float v = f == 0.0f ? 0.0f : acc[k] * f;
+        if (bad) v = __int_as_float(0x7FC00000);
+        out[o + k] = __float2bfloat16_rn(v);
+        if (out_f32) out_f32[o + k] = v;
     }
 }
 
