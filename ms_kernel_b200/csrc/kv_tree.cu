@@ -12,8 +12,8 @@ struct TreePlan {
     int S, key_tile, groups, rows;
 };
 
-// The tuned kernel: head_dim 128, gs = 2, planes on 16-byte boundaries.
-bool umma_eligible(int64_t D, int gs) { return D == 128 && gs == 2; }
+// The tuned kernel: head_dim 128, gs = 2, capacity a multiple of 16, planes on 16-byte boundaries (bulk copies).
+bool umma_eligible(int64_t D, int gs, int64_t Lcap) { return D == 128 && gs == 2 && Lcap % 16 == 0; }
 
 // Rows per thread block by the rows there are; as many runs of the line of tiles as there are SMs, or as
 // there can be tiles.
@@ -30,7 +30,7 @@ TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk
 template <int U, int NR>
 int launch_tree_umma_rows(const KvTreeArgs& a, const TreePlan& p, int B, __nv_bfloat16* out, float* out_f32, cudaStream_t st) {
     static bool configured[64] = {};
-    constexpr int smem = ktu_smem_bytes(NR);
+    constexpr int smem = ktu_smem_bytes(U, NR);
     const int dev = current_device();
     if (dev >= 0 && dev < 64 && !configured[dev]) {
         if (cudaFuncSetAttribute(kv_tree_umma_kernel<U, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
@@ -132,8 +132,8 @@ extern "C" int msaq_kv_tree_attention(const void* q, const int8_t* ks, const uin
         return fail(MSAQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool tuned = umma_eligible(D, gs) &&
-                       !((reinterpret_cast<uintptr_t>(ku) | reinterpret_cast<uintptr_t>(kh) | reinterpret_cast<uintptr_t>(vu) |
+    const bool tuned = umma_eligible(D, gs, Lcap) &&
+                       !((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs) | reinterpret_cast<uintptr_t>(ku) | reinterpret_cast<uintptr_t>(kh) | reinterpret_cast<uintptr_t>(vu) |
                           reinterpret_cast<uintptr_t>(vh)) & 15) &&
                        !(reinterpret_cast<uintptr_t>(q) & 7);
     const TreePlan p = tuned ? plan_tree_umma(B, T, H, Hkv, Lk) : plan_tree_generic(B, T, H, Hkv, Lk);

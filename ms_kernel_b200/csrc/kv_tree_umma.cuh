@@ -4,22 +4,22 @@
 // the tensor cores' wide side:
 //     S^T[128 keys x rows] = K[128 x 128] . Q^T          P^T = 2^(S^T - m)          O^T[128 channels x rows] += V^T . P^T
 // so that the tensor and exponential work follow the number of rows and every thread of the softmax owns one key (its scale is one
-// register).
-//   * Eight decode warps, thread = (key, two 32-blocks): codes go from global memory to registers one tile ahead.  Keys become fp16
-//     operands q 2^(e - e_max) relative to the largest exponent of THEIR row (exact down to 2^-24, 2^-31 of the row's largest
-//     value below) and go to tensor memory as operand A; the factor 2^e_max is applied to the scores.  A block's codes are
-//     8-bit integers offset to bytes: a byte permute drops two of them into the mantissas of 1024.0, one fused multiply-add
-//     takes the offset out and the scale in.  Values become fp16 operands q 2^(e + 2) in shared memory, [key][channel] with the
-//     channel as the contiguous (M) dimension.
-//   * A tile that holds a value block outside the exponents -26 .. 3 (2^-20 to 2^10 in magnitude) is done in bf16 instead, values and
-//     probabilities: the range of fp32 at eight digits, so that a row is not touched by the range of a key it does not see.
-//   * Queries are staged once per item, rotated in fp32, each row scaled by a power of two into fp16 (11 digits; the bf16 query
-//     has 8, its rotation more).  Probabilities are fp16 (11 digits), 2^7 above the reference's scale so that they reach down to 2^-31.
+// register).  The roles meet on mbarriers:
+//   * One warp brings the packed bytes of a tile (25 to 29 bytes per key and 32-block) into a ring in shared memory with TMA bulk
+//     copies, three or four tiles ahead (with one tile ahead in registers the loads' latency alone held the kernel to 2.4 TB/s).
+//   * Two teams of four decode warps take alternate tiles, thread = key.  Keys become fp16 operands q 2^(e - e_max) relative to the
+//     largest exponent of THEIR row (exact down to 2^-24, 2^-31 of the row's largest value below) and go to tensor memory as
+//     operand A; the factor 2^e_max is applied to the scores.  Values become fp16 operands q 2^(e + 1) in shared memory,
+//     [key][channel] with the channel as the contiguous (M) dimension.
+//   * One warp looks at a tile's value exponents first: a tile that holds one outside -25 .. 3 (2^-19 to 2^10 in magnitude) is done
+//     in bf16 instead, values and probabilities: the range of fp32 at eight digits, so that a row is not touched by the range
+//     of a key it does not see.  (Exponents from -100 down, the quantiser's for a block of zeros among them, count as zeros beside the others.)
+//   * Queries are staged once per item, rotated in fp32, scaled by a power of two into fp16 (11 digits; the bf16 query has 8, its
+//     rotation more).  Probabilities are fp16 (11 digits), 2^7 above the reference's scale so that they reach down to 2^-31.
 //   * Eight softmax warps, thread = (key, half of the rows).  The maximum is lazy: a row's reference moves only when a score
 //     exceeds it by more than 2^8 -- one vote per tile of the four warps that hold the row -- and then the accumulators of the
 //     rows concerned are rescaled in tensor memory.  Sums and accumulators are fp32.
-//   * One warp issues the MMAs: S(i + 1) before P.V(i), so that both run under the decoding and the softmax.  Scores, key operands and
-//     probabilities have two buffers, values three; the roles meet on mbarriers only.
+//   * One warp issues the MMAs: S(i + 1) before P.V(i), so that both run under the decoding and the softmax.
 //   * The tiles of all (sequence, kv head, row group) items form one line, cut into equal runs, one per thread block: ragged
 //     batches balance.  An item inside one run is finished there; one that is cut leaves partial results (acc, m, l), merged by a second
 //     kernel in the order of the runs.
@@ -34,13 +34,18 @@
 
 namespace msaq {
 
-constexpr int KTU_WARPS = 8;                                                        // of each of the two working roles
-constexpr int KTU_THREADS = (2 * KTU_WARPS + 1) * 32, KTU_KEYS = 128, KTU_ROWS = 64, KTU_VBUFS = 3;
+constexpr int KTU_WARPS = 8;                                                        // of the decoding, of the softmax
+constexpr int KTU_WARP_MMA = 2 * KTU_WARPS, KTU_WARP_COPY = KTU_WARP_MMA + 1, KTU_WARP_SCOUT = KTU_WARP_MMA + 2, KTU_ALL_WARPS = KTU_WARP_MMA + 3;
+constexpr int KTU_THREADS = KTU_ALL_WARPS * 32, KTU_KEYS = 128, KTU_ROWS = 64;
 constexpr int KTU_COL_O = 0, KTU_COL_S = 64, KTU_COL_K = 192, KTU_COLS = 512;       // tensor memory columns: O, two S, two K (320 used)
-constexpr int KTU_V = 0, KTU_P = KTU_VBUFS * 32768, KTU_Q = KTU_P + 2 * 16384;       // shared memory: values, probabilities, queries
+constexpr int KTU_V = 0, KTU_P = 2 * 32768, KTU_Q = KTU_P + 2 * 16384;               // shared memory: values, probabilities, queries, ring
 constexpr int KTU_PART = 132;                                                       // floats of a row's partial result: acc, m, l, padding
-__host__ __device__ constexpr int ktu_smem_bytes(int nr) { return KTU_Q + nr * 256 + 1024; }
-constexpr int KTU_V_BITS = 2;                                                       // values are held times 2^2
+__host__ __device__ constexpr int ktu_ub(int u) { return 4 * (8 - u); }              // bytes of a block: upper codes, shared codes (and an exponent)
+__host__ __device__ constexpr int ktu_sb(int u) { return 2 * u; }
+__host__ __device__ constexpr int ktu_stages(int u) { return u == 4 ? 4 : 3; }
+__host__ __device__ constexpr int ktu_stage_bytes(int u) { return 2 * 4 * KTU_KEYS * (ktu_ub(u) + ktu_sb(u) + 1); }
+__host__ __device__ constexpr int ktu_smem_bytes(int u, int nr) { return KTU_Q + nr * 256 + ktu_stages(u) * ktu_stage_bytes(u) + 1024; }
+constexpr int KTU_V_BITS = 1;                                                       // values are held times 2
 constexpr float KTU_P_BITS = 7.0f, KTU_MOVE = 15.0f;                                // 2^7 at the reference, which moves at 2^15
 
 // Upper half of a shared-memory matrix descriptor with 128-byte swizzle; the lower half is umma_desc_lo(address, lbo).
@@ -158,87 +163,115 @@ template <> struct KtuRaw<4> { uint4 u; uint2 s; };
 template <> struct KtuRaw<3> { uint32_t u[5]; uint32_t s0, s1; };
 template <> struct KtuRaw<2> { uint2 u[3]; uint32_t s; };
 
-// The bytes of one block.
-__device__ __forceinline__ void ktu_load(KtuRaw<4>& r, const uint8_t* up, const uint8_t* sh) {
-    r.u = __ldcg(reinterpret_cast<const uint4*>(up));
-    r.s = __ldcg(reinterpret_cast<const uint2*>(sh));
+// The bytes of one block: up, sh are shared-memory addresses of this key's codes.
+__device__ __forceinline__ void ktu_load(KtuRaw<4>& r, uint32_t up, uint32_t sh) {
+    r.u = lds128(up);
+    r.s = lds64<0>(sh);
 }
-__device__ __forceinline__ void ktu_load(KtuRaw<3>& r, const uint8_t* up, const uint8_t* sh) {
+__device__ __forceinline__ void ktu_load(KtuRaw<3>& r, uint32_t up, uint32_t sh) {
 #pragma unroll
-    for (int k = 0; k < 5; ++k) r.u[k] = __ldca(reinterpret_cast<const uint32_t*>(up) + k);
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(sh);
-    r.s0 = __ldca(h) | (uint32_t)__ldca(h + 1) << 16;
-    r.s1 = __ldca(h + 2);
+    for (int k = 0; k < 5; ++k) r.u[k] = lds32<0>(up + 4 * k);
+    uint32_t x, y, z;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=r"(x) : "r"(sh));
+    asm volatile("ld.shared.u16 %0, [%1+2];" : "=r"(y) : "r"(sh));
+    asm volatile("ld.shared.u16 %0, [%1+4];" : "=r"(z) : "r"(sh));
+    r.s0 = x | y << 16;
+    r.s1 = z;
 }
-__device__ __forceinline__ void ktu_load(KtuRaw<2>& r, const uint8_t* up, const uint8_t* sh) {
+__device__ __forceinline__ void ktu_load(KtuRaw<2>& r, uint32_t up, uint32_t sh) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) r.u[k] = __ldca(reinterpret_cast<const uint2*>(up) + k);
-    r.s = __ldcg(reinterpret_cast<const uint32_t*>(sh));
-}
-__device__ __forceinline__ void ktu_clear(KtuRaw<4>& r) { r.u = make_uint4(0u, 0u, 0u, 0u); r.s = make_uint2(0u, 0u); }
-__device__ __forceinline__ void ktu_clear(KtuRaw<3>& r) {
-#pragma unroll
-    for (int i = 0; i < 5; ++i) r.u[i] = 0u;
-    r.s0 = r.s1 = 0u;
-}
-__device__ __forceinline__ void ktu_clear(KtuRaw<2>& r) { r.u[0] = r.u[1] = r.u[2] = make_uint2(0u, 0u); r.s = 0u; }
-__device__ __forceinline__ bool ktu_zero(const KtuRaw<4>& r) { return (r.u.x | r.u.y | r.u.z | r.u.w | r.s.x | r.s.y) == 0u; }
-__device__ __forceinline__ bool ktu_zero(const KtuRaw<3>& r) { return (r.u[0] | r.u[1] | r.u[2] | r.u[3] | r.u[4] | r.s0 | r.s1) == 0u; }
-__device__ __forceinline__ bool ktu_zero(const KtuRaw<2>& r) {
-    return (r.u[0].x | r.u[0].y | r.u[1].x | r.u[1].y | r.u[2].x | r.u[2].y | r.s) == 0u;
+    for (int k = 0; k < 3; ++k) r.u[k] = lds64<0>(up + 8 * k);
+    r.s = lds32<0>(sh);
 }
 
-// Codes 8i .. 8i + 7 of a block as offset integers q + 128 + 2^(U-1), bytes 0 and 2 of the words of w: the mantissas of the fp16
-// numbers 1024 + ...  Order inside the eight: U = 4: 0 2, 4 6, 1 3, 5 7 (ktu_place), else as they are.
-template <int U> __device__ __forceinline__ void ktu_codes(const KtuRaw<U>& r, int i, uint32_t (&w)[4]);
-template <> __device__ __forceinline__ void ktu_codes<4>(const KtuRaw<4>& r, int i, uint32_t (&w)[4]) {
-    const uint32_t x = i == 0 ? r.u.x : i == 1 ? r.u.y : i == 2 ? r.u.z : r.u.w, s = i < 2 ? r.s.x : r.s.y;
-    // the four shared codes of these elements (two elements each), one per byte; the sign bits of both codes flipped on the way
-    const uint32_t t = prmt(s, 0u, (i & 1) ? 0x3322u : 0x1100u);
-    const uint32_t lo = and_xor(t >> 4, 0x0F000F00u, and_xor(t, 0x000F000Fu, 0x88888888u));
-    const uint32_t e = and_xor(x << 4, 0xF0F0F0F0u, lo), o = and_xor(x, 0xF0F0F0F0u, lo);
-    w[0] = prmt(e, 0x64646464u, 0x4140u);
-    w[1] = prmt(e, 0x64646464u, 0x4342u);
-    w[2] = prmt(o, 0x64646464u, 0x4140u);
-    w[3] = prmt(o, 0x64646464u, 0x4342u);
+// ---- codes to fp16 -------------------------------------------------------------------------------
+// The 32 values q s of a block (s a power of two up to 2^4 in both halves), eight to a chunk: emit(chunk, four words of two).
+//
+// q = 2^U (U' - 2^(7-U)) + (S' - 2^(U-1)) with both fields' sign bits flipped.  A field that lies in the mantissa of a fp16 number of
+// exponent 2^k, its lowest bit worth 1, reads as 2^k + field: with U' + 64 (or 32) and S' + 1024 (or 16, 64)
+//     A = (S' + 2^j) s - c s,    q s = (U' + 2^k) (2^U s) + A
+// are two fused multiply-adds, the first shared by the two elements of a pair, with every intermediate exact (at most 2184 s).  The
+// logic unit takes an instruction per two cycles and is what bounds the decoding: 8 (U = 4), 12 (U = 3) and 14 (U = 2) of its
+// instructions go into eight elements here, where bytes assembled first and then permuted into mantissas took 11, 33 and 33.
+__device__ __forceinline__ uint32_t hset2(float x) {
+    const __half2 h = __float2half2_rn(x);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <int U> __device__ __forceinline__ void ktu_codes_fields(const uint32_t* up, uint32_t s0, uint32_t s1, int i, uint32_t (&w)[4]) {
-    constexpr int WB = 8 - U;
-    constexpr uint32_t SM = (1u << U) - 1u, UM = ((1u << WB) - 1u) << U;
+__device__ __forceinline__ uint32_t halves(uint32_t lo, uint32_t hi) {        // low half of lo, high half of hi
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, 0xFFFF0000, 0xE4;" : "=r"(r) : "r"(hi), "r"(lo));
+    return r;
+}
+template <int U, typename F> __device__ __forceinline__ void ktu_convert(const KtuRaw<U>& r, uint32_t s, F emit);
+
+// Words of a chunk: elements (0 4) (1 5) (2 6) (3 7).
+template <int U, typename F> __device__ __forceinline__ void ktu_convert_nibbles(const KtuRaw<4>& r, uint32_t s, F emit) {
+    const uint32_t s16 = hmul2(s, 0x4C004C00u), c0 = hmul2(s, hset2(-2184.0f)), c1 = hmul2(s, hset2(-1224.0f));
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const int g = 4 * i + b, ps = g * U;
-        const uint32_t sf = (ps + U <= 32 ? s0 >> ps : ps >= 32 ? s1 >> (ps - 32) : __funnelshift_r(s0, s1, ps)) & SM;
-        uint32_t f[2];
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t x = c == 0 ? r.u.x : c == 1 ? r.u.y : c == 2 ? r.u.z : r.u.w;
+        const uint32_t y = prmt(c < 2 ? r.s.x : r.s.y, 0u, (c & 1) ? 0x4342u : 0x4140u);         // shared codes 1 0 | 3 2
+        const uint32_t a0 = hfma2(and_xor(y, 0x000F000Fu, 0x64086408u), s, c0), a1 = hfma2(and_xor(y, 0x00F000F0u, 0x54805480u), s, c1);
+        const uint32_t x8 = x >> 8;
+        emit(c, hfma2(and_xor(x * 16u, 0x00F000F0u, 0x54805480u), s16, a0), hfma2(and_xor(x, 0x00F000F0u, 0x54805480u), s16, a0),
+             hfma2(and_xor(x8 * 16u, 0x00F000F0u, 0x54805480u), s16, a1), hfma2(and_xor(x8, 0x00F000F0u, 0x54805480u), s16, a1));
+    }
+}
+template <int U> __device__ __forceinline__ uint32_t ktu_window(const uint32_t* w, int bit) {       // 32 bits of the run from `bit` on
+    return (bit & 31) == 0 ? w[bit >> 5] : __funnelshift_r(w[bit >> 5], w[(bit >> 5) + 1], bit & 31);
+}
+// Words of a chunk: elements (0 2) (1 3) (4 6) (5 7).
+template <int U, typename F> __device__ __forceinline__ void ktu_convert_five(const uint32_t (&w)[6], uint32_t s0, uint32_t s1, uint32_t s, F emit) {
+    const uint32_t s8 = hmul2(s, 0x48004800u), c0 = hmul2(s, hset2(-1412.0f)), c1 = hmul2(s, hset2(-404.0f));
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int pk = (2 * g + t) * WB, wi = pk >> 5, po = pk & 31;
-            const uint32_t v = po + WB <= 32 ? up[wi] >> po : __funnelshift_r(up[wi], up[wi + 1], po);
-            f[t] = (v << U) & UM;
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t t = c == 0 ? s0 : c == 1 ? s0 >> 12 : c == 2 ? __funnelshift_r(s0, s1, 24) : s1 >> 4;      // shared codes 4c ..
+        const uint32_t ts = halves(t, t * 8192u);                                                  // 0 2 | 1 3 at bits 0, 6
+        uint32_t o[4];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const uint32_t x = ktu_window<U>(w, 40 * c + 20 * g), y = halves(x, x * 64u);          // 1 0 | 3 2
+            const uint32_t a = g == 0 ? hfma2(and_xor(ts, 0x00070007u, 0x64046404u), s, c0) : hfma2(and_xor(ts, 0x01C001C0u, 0x4D004D00u), s, c1);
+            o[2 * g] = hfma2(and_xor(y * 32u, 0x03E003E0u, 0x52005200u), s8, a);
+            o[2 * g + 1] = hfma2(and_xor(y, 0x03E003E0u, 0x52005200u), s8, a);
         }
-        w[b] = prmt(f[0], f[1], 0x5410u) | ((sf | 0x6400u) * 0x00010001u);
+        emit(c, o[0], o[1], o[2], o[3]);
     }
 }
-template <> __device__ __forceinline__ void ktu_codes<3>(const KtuRaw<3>& r, int i, uint32_t (&w)[4]) {
-    uint32_t up[6];
+template <int U, typename F> __device__ __forceinline__ void ktu_convert_six(const uint32_t (&w)[7], uint32_t sw, uint32_t s, F emit) {
+    const uint32_t s4 = hmul2(s, 0x44004400u), c0 = hmul2(s, hset2(-1410.0f)), c1 = hmul2(s, hset2(-450.0f));
 #pragma unroll
-    for (int k = 0; k < 5; ++k) up[k] = r.u[k] ^ field_signs(5, k);
-    up[5] = 0u;
-    ktu_codes_fields<3>(up, r.s0 ^ field_signs(3, 0), r.s1 ^ (field_signs(3, 1) & 0xFFFFu), i, w);
-}
-template <> __device__ __forceinline__ void ktu_codes<2>(const KtuRaw<2>& r, int i, uint32_t (&w)[4]) {
-    uint32_t up[7];
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t t = sw >> (8 * c), ts = halves(t, t * 16384u);                              // 0 2 | 1 3 at bits 0, 4
+        uint32_t o[4];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        up[2 * k] = r.u[k].x ^ field_signs(6, 2 * k);
-        up[2 * k + 1] = r.u[k].y ^ field_signs(6, 2 * k + 1);
+        for (int g = 0; g < 2; ++g) {
+            const uint32_t x = ktu_window<U>(w, 48 * c + 24 * g), y = halves(x, x * 16u);          // 1 0 | 3 2
+            const uint32_t a = g == 0 ? hfma2(and_xor(ts, 0x00030003u, 0x64026402u), s, c0) : hfma2(and_xor(ts, 0x00300030u, 0x54205420u), s, c1);
+            o[2 * g] = hfma2(and_xor(y * 16u, 0x03F003F0u, 0x56005600u), s4, a);
+            o[2 * g + 1] = hfma2(and_xor(y >> 2, 0x03F003F0u, 0x56005600u), s4, a);
+        }
+        emit(c, o[0], o[1], o[2], o[3]);
     }
-    up[6] = 0u;
-    ktu_codes_fields<2>(up, r.s ^ field_signs(2, 0), 0u, i, w);
+}
+template <int U, typename F> __device__ __forceinline__ void ktu_convert(const KtuRaw<U>& r, uint32_t s, F emit) {
+    if constexpr (U == 4) {
+        ktu_convert_nibbles<U>(r, s, emit);
+    } else if constexpr (U == 3) {
+        const uint32_t w[6] = {r.u[0], r.u[1], r.u[2], r.u[3], r.u[4], 0u};
+        ktu_convert_five<U>(w, r.s0, r.s1, s, emit);
+    } else {
+        const uint32_t w[7] = {r.u[0].x, r.u[0].y, r.u[1].x, r.u[1].y, r.u[2].x, r.u[2].y, 0u};
+        ktu_convert_six<U>(w, r.s, s, emit);
+    }
 }
 // Where element e of a row is among the operands, and back.
-template <int U> __host__ __device__ __forceinline__ int ktu_place(int e) { return U == 4 ? (e & ~7) | (e & 1) << 2 | (e >> 1 & 3) : e; }
-template <int U> __host__ __device__ __forceinline__ int ktu_element(int p) { return U == 4 ? (p & ~7) | (p >> 2 & 1) | (p & 3) << 1 : p; }
+template <int U> __host__ __device__ __forceinline__ int ktu_place(int e) {
+    return U == 4 ? (e & ~7) | (e & 3) << 1 | (e >> 2 & 1) : (e & ~3) | (e & 1) << 1 | (e >> 1 & 1);
+}
+template <int U> __host__ __device__ __forceinline__ int ktu_element(int p) {
+    return U == 4 ? (p & ~7) | (p >> 1 & 3) | (p & 1) << 2 : (p & ~3) | (p & 1) << 1 | (p >> 1 & 1);
+}
 
 // ---- the line of tiles -------------------------------------------------------------------------
 // Item (b, hk, group) has tiles_of(b) tiles; items in that order, sequences first.  Of the N tiles thread block c of C <= N takes
@@ -322,13 +355,14 @@ template <int N> __device__ __forceinline__ void ktu_column_sums(float (&v)[N], 
 }
 
 struct __align__(16) KtuShared {
-    uint64_t kfull[4], vfull[KTU_VBUFS], sfull[2], pfull[2], qfull[4];        // written: keys, values, scores, probabilities, queries
-    uint64_t sempty[2], vempty[KTU_VBUFS], pempty[2], done;                   // read
+    uint64_t rfull[4], rempty[4], ready[4];                                   // ring: bytes landed, read, looked at
+    uint64_t kfull[4], vfull[2], sfull[2], pfull[2], qfull[4];                // written: keys, values, scores, probabilities, queries
+    uint64_t sempty[2], vempty[2], pempty[2], done;                           // read
     uint32_t tmem;
     int seq;
-    long long seq_tile, red[2 * (2 * KTU_WARPS + 1)];
+    long long seq_tile, red[2 * KTU_ALL_WARPS];
     volatile int abort;
-    int wide[4];                                                  // tile's values (and probabilities) are bf16
+    int wide[8];                                                  // tile's values (and probabilities) are bf16
     uint64_t mask[KT_MAX_T];
     float qf[4][KTU_ROWS], qscale[4];                             // score factors 2^x of the query rows; of all rows where they are the same
     int same[4], qtop[KTU_WARPS], qlow[KTU_WARPS];
@@ -343,20 +377,19 @@ __global__ void __launch_bounds__(KTU_THREADS, 1)
 kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32) {
     chain_wait();
     constexpr int NC = NR / 2;                                    // columns (query rows) of a thread in the softmax
-    constexpr uint32_t OFFSET = 1024u + 128u + (1u << (U - 1));   // what the mantissa bytes stand above the codes
     extern __shared__ uint8_t ktu_smem_raw[];
     __shared__ KtuShared sh;
     const uint32_t sbase = (smem_u32(ktu_smem_raw) + 1023u) & ~1023u;
     uint8_t* const smem = ktu_smem_raw + (sbase - smem_u32(ktu_smem_raw));
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int role = warp / KTU_WARPS, quad = warp & 3, half = warp >> 2 & 1;      // role 0: decode, 1: softmax, 2: MMAs
+    const int role = warp / KTU_WARPS, quad = warp & 3, half = warp >> 2 & 1;      // role 0: decode (half: team), 1: softmax, 2: the single warps
     const int key = quad * 32 + lane;                             // this thread's key of a tile
     const int G = a.Hq / a.Hkv, R = a.T * G, per_seq = a.Hkv * groups;
 
     // ---- this thread block's run of tiles, and where it begins ----
     int64_t skip, total;
-    ktu_sums<2 * KTU_WARPS + 1>(a, B, 0, sh.red, &skip, &total);
+    ktu_sums<KTU_ALL_WARPS>(a, B, 0, sh.red, &skip, &total);
     total *= per_seq;
     const int C = (int)min((int64_t)gridDim.x, total);            // no run is empty
     if ((int)blockIdx.x >= C) return;
@@ -377,17 +410,24 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             if (base > g0) break;
         }
     }
-    if (role == 2) {
+    if (warp == KTU_WARP_MMA) {
         tmem_alloc(smem_u32(&sh.tmem), KTU_COLS);
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < 4; ++i) { mbar_init(smem_u32(&sh.kfull[i]), KTU_WARPS); mbar_init(smem_u32(&sh.qfull[i]), KTU_WARPS); }
-        for (int i = 0; i < KTU_VBUFS; ++i) { mbar_init(smem_u32(&sh.vfull[i]), KTU_WARPS); mbar_init(smem_u32(&sh.vempty[i]), 1); }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_u32(&sh.rfull[i]), 1);
+            mbar_init(smem_u32(&sh.rempty[i]), 4);
+            mbar_init(smem_u32(&sh.ready[i]), 1);
+            mbar_init(smem_u32(&sh.kfull[i]), 4);
+            mbar_init(smem_u32(&sh.qfull[i]), KTU_WARPS);
+        }
         for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh.vfull[i]), 4);
             mbar_init(smem_u32(&sh.sfull[i]), 1);
             mbar_init(smem_u32(&sh.pfull[i]), KTU_WARPS);
             mbar_init(smem_u32(&sh.sempty[i]), KTU_WARPS);
+            mbar_init(smem_u32(&sh.vempty[i]), 1);
             mbar_init(smem_u32(&sh.pempty[i]), 1);
         }
         mbar_init(smem_u32(&sh.done), 1);
@@ -408,6 +448,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     }
     const KtuCursor start = cur;
 
+    constexpr int UB = ktu_ub(U), SB = ktu_sb(U), NST = ktu_stages(U);
+    constexpr int K_SH = 4 * KTU_KEYS * UB, K_SC = K_SH + 4 * KTU_KEYS * SB, V_UP = K_SC + 4 * KTU_KEYS, V_SH = V_UP + K_SH, V_SC = V_UP + K_SC;
+    const uint32_t ring = sbase + KTU_Q + NR * 256;               // stages: upper, shared codes and exponents of the keys, of the values
+    const uint32_t vrow = (sbase + KTU_V + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;      // with the swizzle of chunk 0
+
     // A bounded wait of the whole warp; false: it ran out, here or elsewhere.  A warp whose wait failed waits no more but goes on through
     // the motions, since others of its role meet it at the named barriers; the outputs are marked in the end.
     auto wait = [&](const uint64_t& bar, uint32_t phase) {
@@ -426,61 +471,8 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
 
     if (role == 0) {
         // ================================ decode ================================
-        KtuRaw<U> kraw[2], vraw[2];
-        int ke[4], ve[2];
-        constexpr int UB = 4 * (8 - U), SB = 2 * U;
-        const int64_t cap = a.Lcap;
-        // this thread's key of the next tile to load, in the planes of blocks 2 half (codes) and 0 (exponents of keys)
-        const uint8_t *ku, *kh, *vu, *vh;
-        const int8_t *ks, *vs;
-        int left;                                                 // keys of the sequence from this thread's one on
-        auto seek = [&](const KtuCursor& c) {
-            const int64_t s0 = ((int64_t)c.b * a.Hkv + c.hk) * 4 * cap + c.t * KTU_KEYS + key, s1 = s0 + 2 * half * cap;
-            ku = a.k.u + s1 * UB;
-            kh = a.k.h + s1 * SB;
-            ks = a.k.s + s0;
-            vu = a.v.u + s1 * UB;
-            vh = a.v.h + s1 * SB;
-            vs = a.v.s + s1;
-            left = c.len + a.T - c.t * KTU_KEYS - key;
-        };
-        auto load_k = [&]() {
-            if (left > 0) {
-                ktu_load(kraw[0], ku, kh);
-                ktu_load(kraw[1], ku + cap * UB, kh + cap * SB);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ke[i] = __ldcg(ks + i * cap);
-            } else {
-                ktu_clear(kraw[0]);
-                ktu_clear(kraw[1]);
-                ke[0] = ke[1] = ke[2] = ke[3] = -127;
-            }
-            ku += KTU_KEYS * UB;
-            kh += KTU_KEYS * SB;
-            ks += KTU_KEYS;
-        };
-        auto load_v = [&]() {
-            if (left > 0) {
-                ktu_load(vraw[0], vu, vh);
-                ktu_load(vraw[1], vu + cap * UB, vh + cap * SB);
-                ve[0] = __ldcg(vs);
-                ve[1] = __ldcg(vs + cap);
-            } else {
-                ktu_clear(vraw[0]);
-                ktu_clear(vraw[1]);
-                ve[0] = ve[1] = 0;
-            }
-            vu += KTU_KEYS * UB;
-            vh += KTU_KEYS * SB;
-            vs += KTU_KEYS;
-            left -= KTU_KEYS;
-        };
-        seek(cur);
-        load_k();
-        load_v();
-        int seg = -1, vbuf = 0;
-        uint32_t vphase = 0;
-        const uint32_t vrow = (half * 16384 + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;     // with the swizzle of chunk 0
+        int seg = -1;
+        uint32_t n_slot = 0, r_phase = 0;                         // the tile's slot of the ring
         bool ok = true;
 #pragma unroll 1
         for (int j = 0; j < n_run; ++j) {
@@ -543,83 +535,68 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 fence_async_smem();
                 arrive(sh.qfull[seg & 3]);
             }
-            // ---- keys to tensor memory, once the product before the last has read the buffer ----
-            if (j > 1) ok = ok && wait(sh.sfull[j & 1], (uint32_t)(j - 2) >> 1);
-            tc_fence_after();
-            const int emax = max(max(ke[0], ke[1]), max(ke[2], ke[3]));
-            if (half == 0) sh.ck[j & 3][key] = a.sm_scale_log2 * exp2_int(emax);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t sc = ktu_pow2_h2((half ? ke[2 + i] : ke[i]) - emax);
-                const uint32_t off = hmul2(sc, 0xE400E400u + (OFFSET - 1024u) * 0x00010001u);  // -OFFSET (fp16 counts in ones from 1024 to 2048)
-                uint32_t w[16];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t t[4];
-                    ktu_codes<U>(kraw[i], c, t);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) w[4 * c + x] = hfma2(t[x], sc, off);
-                }
-                ktu_st16(tlane + KTU_COL_K + (j & 1) * 64 + half * 32 + i * 16, w);
-            }
+            const uint32_t slot = n_slot, phase = r_phase;
+            if (++n_slot == NST) { n_slot = 0; r_phase ^= 1u; }
             cur.next(a, groups, B);
-            if (j + 1 < n_run) {
-                if (cur.t == 0) seek(cur);
-                load_k();
+            if ((j & 1) != half) continue;                        // the other team's tile
+            ok = ok && wait(sh.rfull[slot], phase);
+            ok = ok && wait(sh.ready[slot], phase);
+            const uint32_t st = ring + slot * ktu_stage_bytes(U);
+            // ---- keys to tensor memory, once the product before the last has read the buffer ----
+            const uint32_t es = lds_s8<K_SC>(st + key) & 0xFF | (lds_s8<K_SC + KTU_KEYS>(st + key) & 0xFF) << 8 |
+                                (lds_s8<K_SC + 2 * KTU_KEYS>(st + key) & 0xFF) << 16 | lds_s8<K_SC + 3 * KTU_KEYS>(st + key) << 24;
+            const int emax = max(max((int)(es << 24) >> 24, (int)(es << 16) >> 24), max((int)(es << 8) >> 24, (int)es >> 24));
+            sh.ck[j & 3][key] = a.sm_scale_log2 * exp2_int(emax);
+            if (j > 1) ok = ok && wait(sh.sfull[half], (uint32_t)(j - 2) >> 1);
+            tc_fence_after();
+            // (block loops stay rolled: the roles' code shares an instruction cache)
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                KtuRaw<U> raw;
+                ktu_load(raw, st + i * KTU_KEYS * UB + key * UB, st + K_SH + i * KTU_KEYS * SB + key * SB);
+                uint32_t w[16];
+                ktu_convert<U>(raw, ktu_pow2_h2(((int)(es << (24 - 8 * i)) >> 24) - emax), [&](int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+                    w[4 * c] = w0; w[4 * c + 1] = w1; w[4 * c + 2] = w2; w[4 * c + 3] = w3;
+                });
+                ktu_st16(tlane + KTU_COL_K + half * 64 + i * 16, w);
             }
             ktu_st_wait();
             tc_fence_before();
             arrive(sh.kfull[j & 3]);
-            // ---- values to shared memory, once the buffer's last product has read them; a block outside the exponents that fp16 holds? ----
-            bool far = (unsigned)(ve[0] + 24 + KTU_V_BITS) > 29u || (unsigned)(ve[1] + 24 + KTU_V_BITS) > 29u;
-            if (far) far = ((unsigned)(ve[0] + 24 + KTU_V_BITS) > 29u && !ktu_zero(vraw[0])) || ((unsigned)(ve[1] + 24 + KTU_V_BITS) > 29u && !ktu_zero(vraw[1]));
-            const bool wide = ktu_vote(1, KTU_WARPS * 32, far);
-            if (tid == 0) sh.wide[j & 3] = wide;
-            if (j >= KTU_VBUFS) ok = ok && wait(sh.vempty[vbuf], vphase ^ 1u);
-            const uint32_t row = sbase + KTU_V + vbuf * 32768 + vrow;
-            if (!wide) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t sc = ktu_pow2_h2(min(max(ve[i], -24 - KTU_V_BITS), 5 - KTU_V_BITS) + KTU_V_BITS);   // (out of range: zeros)
-                    const uint32_t off = hmul2(sc, 0xE400E400u + (OFFSET - 1024u) * 0x00010001u);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t t[4];
-                        ktu_codes<U>(vraw[i], c, t);
-                        sts128(row ^ (i * 4 + c) << 4, hfma2(t[0], sc, off), hfma2(t[1], sc, off), hfma2(t[2], sc, off),
-                               hfma2(t[3], sc, off));
-                    }
-                }
-            } else {
+            // ---- values to shared memory, once the product before the last has read them ----
+            if (j > 1) ok = ok && wait(sh.vempty[half], (uint32_t)(j - 2) >> 1);
+            const uint32_t row = vrow + half * 32768;
+            const bool wide = sh.wide[j & 7] != 0;
 #pragma unroll 1
-                for (int i = 0; i < 2; ++i) {
-                    const float sc = exp2_int(max(-126, min(116, (i ? ve[1] : ve[0]) + KTU_V_BITS)));
-                    const KtuRaw<U> raw = i ? vraw[1] : vraw[0];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t t[4];
-                        ktu_codes<U>(raw, c, t);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float f0 = (float)((int)(t[x] & 0xFFu) - (int)(OFFSET - 1024u)) * sc;
-                            const float f1 = (float)((int)(t[x] >> 16 & 0xFFu) - (int)(OFFSET - 1024u)) * sc;
-                            t[x] = prmt(__float_as_uint(f0), __float_as_uint(f1), 0x7632u);      // eight digits: exact
-                        }
-                        sts128(row ^ (i * 4 + c) << 4, t[0], t[1], t[2], t[3]);
-                    }
+            for (int i = 0; i < 4; ++i) {
+                KtuRaw<U> raw;
+                ktu_load(raw, st + V_UP + i * KTU_KEYS * UB + key * UB, st + V_SH + i * KTU_KEYS * SB + key * SB);
+                const int ve = lds_s8<V_SC>(st + i * KTU_KEYS + key);
+                const uint32_t at = row + (i >> 1) * 16384;
+                if (!wide) {
+                    // (out of range: zeros, or a key that no row attends)
+                    ktu_convert<U>(raw, ktu_pow2_h2(min(max(ve, -100), 4 - KTU_V_BITS) + KTU_V_BITS),
+                                   [&](int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) { sts128(at ^ ((i & 1) * 4 + c) << 4, w0, w1, w2, w3); });
+                } else {
+                    const float sc = exp2_int(max(-126, min(116, ve + KTU_V_BITS)));
+                    const auto bf = [&](uint32_t w) {                         // eight digits: exact
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                        return prmt(__float_as_uint(f.x * sc), __float_as_uint(f.y * sc), 0x7632u);
+                    };
+                    ktu_convert<U>(raw, 0x3C003C00u, [&](int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+                        sts128(at ^ ((i & 1) * 4 + c) << 4, bf(w0), bf(w1), bf(w2), bf(w3));
+                    });
                 }
             }
-            if (j + 1 < n_run) load_v();
+            arrive(sh.rempty[slot]);
             fence_async_smem();
-            arrive(sh.vfull[vbuf]);
-            if (++vbuf == KTU_VBUFS) { vbuf = 0; vphase ^= 1u; }
+            arrive(sh.vfull[half]);
         }
     } else if (role == 1) {
         // ================================ softmax ================================
         const uint32_t prow = (sbase + KTU_P + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;
         const int stid = tid - KTU_WARPS * 32, htid = stid & 127;             // thread of the role, of its half
-        int seg = -1, n_seg = 0, vbuf = 0;
-        uint32_t vphase = 0;
+        int seg = -1, n_seg = 0;
         bool ok = true;
         bool same = true;                                         // the item's query rows have one score factor
         float qscale = 1.0f;
@@ -649,6 +626,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             const bool tail = jb + KTU_KEYS > cur.len;            // the tile has nodes of the tree
             ok = ok && wait(sh.kfull[j & 3], (uint32_t)j >> 2);
             const float ck = same ? sh.ck[j & 3][key] * qscale : sh.ck[j & 3][key];
+            const bool wide = sh.wide[j & 7] != 0;
             uint32_t vis = 0xFFFFFFFFu;                           // which of this thread's rows attend its key
             if (tail) {
                 const int k = jb + key - cur.len;                 // below 0: in front of the tree
@@ -682,17 +660,20 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     for (int c = 0; c < NC; ++c)
                         if (!(vis >> c & 1)) x[c] = -INFINITY;
             };
-            scores();
-            float top = x[0], top1 = x[1];
-#pragma unroll
-            for (int c = 2; c < NC; c += 2) {
-                top = fmaxf(top, x[c]);
-                top1 = fmaxf(top1, x[c + 1]);
-            }
-            top = fmaxf(top, top1);
             // the product before the last has read this tile's buffer of the probabilities
             if (j > 1) ok = ok && wait(sh.pempty[j & 1], (uint32_t)(j - 2) >> 1);
-            if (ktu_vote(3 + half, KTU_WARPS * 16, n_seg == 0 || top > KTU_MOVE)) {
+            bool moved = false;
+#pragma unroll 1
+            for (;;) {
+                scores();
+                float top = x[0], top1 = x[1];
+#pragma unroll
+                for (int c = 2; c < NC; c += 2) {
+                    top = fmaxf(top, x[c]);
+                    top1 = fmaxf(top1, x[c + 1]);
+                }
+                if (moved || !ktu_vote(3 + half, KTU_WARPS * 16, n_seg == 0 || fmaxf(top, top1) > KTU_MOVE)) break;
+                moved = true;
                 // ---- references move: rows of this half whose maximum of this tile is beyond theirs ----
                 if (n_seg > 0) ok = ok && wait(sh.pempty[(j - 1) & 1], (uint32_t)(j - 1) >> 1);  // the accumulators are at rest
 #pragma unroll 1
@@ -745,31 +726,26 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     }
                     ktu_st_wait();
                 }
-                scores();
             }
             tc_fence_before();
             arrive(sh.sempty[j & 1]);
             // ---- probabilities to shared memory, in the type of the tile's values ----
-            ok = ok && wait(sh.vfull[vbuf], vphase);
-            const bool wide = sh.wide[j & 3] != 0;
-            if (++vbuf == KTU_VBUFS) { vbuf = 0; vphase ^= 1u; }
             const uint32_t pr = prow + (j & 1) * 16384;
-            auto store_p = [&](auto bf16) {
 #pragma unroll
-                for (int c = 0; c < NC; c += 8) {
-                    uint32_t w[4];
+            for (int c = 0; c < NC; c += 8) {
+                uint32_t w[4];
 #pragma unroll
-                    for (int k = 0; k < 8; k += 2) {
-                        const float p0 = ktu_exp2(x[c + k]), p1 = ktu_exp2(x[c + k + 1]);
-                        l[(c + k) / 2] = add2(l[(c + k) / 2], pack2(p0, p1));
-                        if constexpr (!decltype(bf16)::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
-                        else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(p1), "f"(p0));
-                    }
-                    sts128(pr ^ (half * (NC / 8) + c / 8) << 4, w[0], w[1], w[2], w[3]);
+                for (int k = 0; k < 8; k += 2) {
+                    x[c + k] = ktu_exp2(x[c + k]);
+                    x[c + k + 1] = ktu_exp2(x[c + k + 1]);
+                    l[(c + k) / 2] = add2(l[(c + k) / 2], pack2(x[c + k], x[c + k + 1]));
+                    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(x[c + k + 1]), "f"(x[c + k]));
                 }
-            };
-            if (wide) store_p(std::true_type{});
-            else store_p(std::false_type{});
+                if (wide)
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(x[c + k + 1]), "f"(x[c + k]));
+                sts128(pr ^ (half * (NC / 8) + c / 8) << 4, w[0], w[1], w[2], w[3]);
+            }
             fence_async_smem();
             tc_fence_before();
             arrive(sh.pfull[j & 1]);
@@ -824,11 +800,10 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             }
             cur.next(a, groups, B);
         }
-    } else {
+    } else if (warp == KTU_WARP_MMA) {
         // ================================ MMAs ================================
         const uint32_t idesc_qk = ktu_idesc(NR, 0, 0), hi = ktu_desc_hi(1024);
-        int seg = -1, vbuf = 0;
-        uint32_t vphase = 0;
+        int seg = -1;
         KtuCursor ahead = cur;                                    // of the scores' product, one tile in front
         auto issue_qk = [&](int j) {
             if (j == 0 || ahead.t == 0) {
@@ -854,19 +829,18 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
 #pragma unroll 1
             for (int j = 0; j < n_run; ++j) {
                 if (j + 1 < n_run && !issue_qk(j + 1)) break;
-                if (!wait(sh.vfull[vbuf], vphase) || !wait(sh.pfull[j & 1], (uint32_t)j >> 1)) break;
+                if (!wait(sh.vfull[j & 1], (uint32_t)j >> 1) || !wait(sh.pfull[j & 1], (uint32_t)j >> 1)) break;
                 tc_fence_after();
-                const uint32_t id = ktu_idesc(NR, sh.wide[j & 3] ? 1u : 0u, 1u);
+                const uint32_t id = ktu_idesc(NR, sh.wide[j & 7] ? 1u : 0u, 1u);
                 if (elect_lane()) {
 #pragma unroll
                     for (int s = 0; s < 8; ++s)
-                        ktu_mma_ss(tm + KTU_COL_O, umma_desc_lo(sbase + KTU_V + vbuf * 32768 + s * 2048, 16384), hi,
+                        ktu_mma_ss(tm + KTU_COL_O, umma_desc_lo(sbase + KTU_V + (j & 1) * 32768 + s * 2048, 16384), hi,
                                    umma_desc_lo(sbase + KTU_P + (j & 1) * 16384 + s * 2048, 8192), hi, id, !first || s > 0);
-                    tc_commit(smem_u32(&sh.vempty[vbuf]));
+                    tc_commit(smem_u32(&sh.vempty[j & 1]));
                     tc_commit(smem_u32(&sh.pempty[j & 1]));
                 }
                 __syncwarp();
-                if (++vbuf == KTU_VBUFS) { vbuf = 0; vphase ^= 1u; }
                 first = cur.t == cur.tiles - 1;
                 cur.next(a, groups, B);
             }
@@ -876,12 +850,56 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             mbar_wait_bounded(smem_u32(&sh.done), 0);
         }
         __syncwarp();
+    } else if (warp == KTU_WARP_COPY) {
+        // ================================ copies ================================
+        // Lane 4 p + i brings plane p (keys: upper, shared, exponents; values: the same) of block i.
+        const int p = lane >> 2, i = lane & 3, kind = p % 3, per_key = kind == 0 ? UB : kind == 1 ? SB : 1;
+        const KvPlanes& pl = p < 3 ? a.k : a.v;
+        const uint8_t* src = kind == 0 ? pl.u : kind == 1 ? pl.h : reinterpret_cast<const uint8_t*>(pl.s);
+        const uint32_t dst = (p < 3 ? 0 : V_UP) + (kind == 0 ? 0 : kind == 1 ? K_SH : K_SC) + i * KTU_KEYS * per_key;
+        uint32_t slot = 0, phase = 1;                             // passes at once on a fresh barrier
+        int issued = 0;
+        for (int j = 0; j < n_run; ++j) {
+            if (!wait(sh.rempty[slot], phase)) break;
+            const int n = min(KTU_KEYS, (cur.len + a.T - cur.t * KTU_KEYS + 15) & ~15);            // whole groups of 16 (so is the capacity)
+            const int64_t row = (((int64_t)cur.b * a.Hkv + cur.hk) * 4 + i) * a.Lcap + cur.t * KTU_KEYS;
+            const uint32_t bar = smem_u32(&sh.rfull[slot]);
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n * 8 * (UB + SB + 1)));
+            __syncwarp();
+            if (lane < 24) bulk_g2s(ring + slot * ktu_stage_bytes(U) + dst, src + row * per_key, (uint32_t)(n * per_key), bar);
+            ++issued;
+            cur.next(a, groups, B);
+            if (++slot == NST) { slot = 0; phase ^= 1u; }
+        }
+        // shared memory is not handed on with a copy in flight
+        for (int j = max(0, issued - NST); j < issued; ++j) mbar_wait_bounded(smem_u32(&sh.rfull[j % NST]), (uint32_t)(j / NST) & 1u);
+        __syncwarp();
+    } else {
+        // ================================ value exponents ================================
+        uint32_t slot = 0, phase = 0;
+        for (int j = 0; j < n_run; ++j) {
+            if (!wait(sh.rfull[slot], phase)) break;
+            const uint4 v = lds128<V_SC>(ring + slot * ktu_stage_bytes(U) + lane * 16);            // block lane / 8, keys 16 (lane % 8) ..
+            const int valid = cur.len + a.T - cur.t * KTU_KEYS - (lane & 7) * 16;
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            bool far = false;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int e = (int)(w[k >> 2] << (24 - 8 * (k & 3))) >> 24;
+                far = far || (k < valid && e > -100 && (unsigned)(e + 24 + KTU_V_BITS) > 28u);
+            }
+            far = __any_sync(0xffffffffu, far);
+            if (lane == 0) sh.wide[j & 7] = far;
+            arrive(sh.ready[slot]);
+            cur.next(a, groups, B);
+            if (++slot == NST) { slot = 0; phase ^= 1u; }
+        }
     }
 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (role == 2) tmem_dealloc(tm, KTU_COLS);
+    if (warp == KTU_WARP_MMA) tmem_dealloc(tm, KTU_COLS);
     if (sh.abort) {
         // a wait gave up: everything of this run is marked
         if (tid == 0) report_wait_failure(a.sticky, WAIT_FAIL_KV_DECODE);
