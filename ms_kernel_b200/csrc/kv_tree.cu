@@ -37,7 +37,7 @@ int launch_tree_umma_rows(const KvTreeArgs& a, const TreePlan& p, int B, __nv_bf
             return fail(MSAQ_ERR_CUDA, "cannot reserve %d bytes of shared memory", smem);
         configured[dev] = true;
     }
-    launch_chained(kv_tree_umma_kernel<U, NR>, dim3((unsigned)p.S), dim3(KTU_THREADS), smem, st, a, B, p.groups, out, out_f32);
+    launch_chained(kv_tree_umma_kernel<U, NR>, dim3((unsigned)p.S), dim3(ktu_threads(NR)), smem, st, a, B, p.groups, out, out_f32);
     count_launch();
     if (int rc = check_launch("kv_tree_umma")) return rc;
     launch_chained(kv_tree_merge_kernel<NR>, dim3((unsigned)(a.Hkv * p.groups * (NR / 8)), (unsigned)B), dim3(256), 0, st, a, B, p.groups, p.S, out,

@@ -7,7 +7,7 @@
 // register).  The roles meet on mbarriers:
 //   * One warp brings the packed bytes of a tile (25 to 29 bytes per key and 32-block) into a ring in shared memory with TMA bulk
 //     copies, three or four tiles ahead (with one tile ahead in registers the loads' latency alone held the kernel to 2.4 TB/s).
-//   * Two teams of four decode warps take alternate tiles, thread = key.  Keys become fp16 operands q 2^(e - e_max) relative to the
+//   * Two teams of eight decode warps take alternate tiles, thread = (key, two 32-blocks).  Keys become fp16 operands q 2^(e - e_max) relative to the
 //     largest exponent of THEIR row (exact down to 2^-24, 2^-31 of the row's largest value below) and go to tensor memory as
 //     operand A; the factor 2^e_max is applied to the scores.  Values become fp16 operands q 2^(e + 1) in shared memory,
 //     [key][channel] with the channel as the contiguous (M) dimension.
@@ -16,7 +16,7 @@
 //     of a key it does not see.  (Exponents from -100 down, the quantiser's for a block of zeros among them, count as zeros beside the others.)
 //   * Queries are staged once per item, rotated in fp32, scaled by a power of two into fp16 (11 digits; the bf16 query has 8, its
 //     rotation more).  Probabilities are fp16 (11 digits), 2^7 above the reference's scale so that they reach down to 2^-31.
-//   * Eight softmax warps, thread = (key, half of the rows).  The maximum is lazy: a row's reference moves only when a score
+//   * Eight softmax warps, thread = (key, half of the rows), four up to 32 rows.  The maximum is lazy: a row's reference moves only when a score
 //     exceeds it by more than 2^8 -- one vote per tile of the four warps that hold the row -- and then the accumulators of the
 //     rows concerned are rescaled in tensor memory.  Sums and accumulators are fp32.
 //   * One warp issues the MMAs: S(i + 1) before P.V(i), so that both run under the decoding and the softmax.
@@ -34,9 +34,10 @@
 
 namespace msaq {
 
-constexpr int KTU_WARPS = 8;                                                        // of the decoding, of the softmax
-constexpr int KTU_WARP_MMA = 2 * KTU_WARPS, KTU_WARP_COPY = KTU_WARP_MMA + 1, KTU_WARP_SCOUT = KTU_WARP_MMA + 2, KTU_ALL_WARPS = KTU_WARP_MMA + 3;
-constexpr int KTU_THREADS = KTU_ALL_WARPS * 32, KTU_KEYS = 128, KTU_ROWS = 64;
+constexpr int KTU_DEC_WARPS = 16, KTU_KEYS = 128, KTU_ROWS = 64;
+// Softmax warps: two halves of the rows by four quarters of the keys; up to 32 rows one set of four (a warp's work is mostly its waits then).
+__host__ __device__ constexpr int ktu_soft_warps(int nr) { return nr > 32 ? 8 : 4; }
+__host__ __device__ constexpr int ktu_threads(int nr) { return (KTU_DEC_WARPS + ktu_soft_warps(nr) + 4) * 32; }       // and four single ones
 constexpr int KTU_COL_O = 0, KTU_COL_S = 64, KTU_COL_K = 192, KTU_COLS = 512;       // tensor memory columns: O, two S, two K (320 used)
 constexpr int KTU_V = 0, KTU_P = 2 * 32768, KTU_Q = KTU_P + 2 * 16384;               // shared memory: values, probabilities, queries, ring
 constexpr int KTU_PART = 132;                                                       // floats of a row's partial result: acc, m, l, padding
@@ -151,7 +152,7 @@ __device__ __forceinline__ float ktu_exp2(float x) {       // 2^x, x <= 15; -inf
     return r;
 }
 
-// 2^d, d <= 15, in both halves; below the smallest fp16 number 0.
+// 2^d, -24 <= d <= 15, in both halves; below 0.
 __device__ __forceinline__ uint32_t ktu_pow2_h2(int d) {
     const uint32_t h = d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
     return h * 0x00010001u;
@@ -202,67 +203,60 @@ __device__ __forceinline__ uint32_t halves(uint32_t lo, uint32_t hi) {        //
     asm("lop3.b32 %0, %1, %2, 0xFFFF0000, 0xE4;" : "=r"(r) : "r"(hi), "r"(lo));
     return r;
 }
-template <int U, typename F> __device__ __forceinline__ void ktu_convert(const KtuRaw<U>& r, uint32_t s, F emit);
-
+// {s, 2^U s, -(2^j) s's of the two kinds of A} for s = 2^d.
+template <int U> __device__ __forceinline__ uint4 ktu_scales(int d) {
+    const uint32_t s = ktu_pow2_h2(d);
+    if (U == 4) return make_uint4(s, hmul2(s, 0x4C004C00u), hmul2(s, hset2(-2184.0f)), hmul2(s, hset2(-1224.0f)));
+    if (U == 3) return make_uint4(s, hmul2(s, 0x48004800u), hmul2(s, hset2(-1412.0f)), hmul2(s, hset2(-404.0f)));
+    return make_uint4(s, hmul2(s, 0x44004400u), hmul2(s, hset2(-1410.0f)), hmul2(s, hset2(-450.0f)));
+}
 // Words of a chunk: elements (0 4) (1 5) (2 6) (3 7).
-template <int U, typename F> __device__ __forceinline__ void ktu_convert_nibbles(const KtuRaw<4>& r, uint32_t s, F emit) {
-    const uint32_t s16 = hmul2(s, 0x4C004C00u), c0 = hmul2(s, hset2(-2184.0f)), c1 = hmul2(s, hset2(-1224.0f));
+template <typename F> __device__ __forceinline__ void ktu_convert(const KtuRaw<4>& r, const uint4& s, F emit) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const uint32_t x = c == 0 ? r.u.x : c == 1 ? r.u.y : c == 2 ? r.u.z : r.u.w;
         const uint32_t y = prmt(c < 2 ? r.s.x : r.s.y, 0u, (c & 1) ? 0x4342u : 0x4140u);         // shared codes 1 0 | 3 2
-        const uint32_t a0 = hfma2(and_xor(y, 0x000F000Fu, 0x64086408u), s, c0), a1 = hfma2(and_xor(y, 0x00F000F0u, 0x54805480u), s, c1);
+        const uint32_t a0 = hfma2(and_xor(y, 0x000F000Fu, 0x64086408u), s.x, s.z), a1 = hfma2(and_xor(y, 0x00F000F0u, 0x54805480u), s.x, s.w);
         const uint32_t x8 = x >> 8;
-        emit(c, hfma2(and_xor(x * 16u, 0x00F000F0u, 0x54805480u), s16, a0), hfma2(and_xor(x, 0x00F000F0u, 0x54805480u), s16, a0),
-             hfma2(and_xor(x8 * 16u, 0x00F000F0u, 0x54805480u), s16, a1), hfma2(and_xor(x8, 0x00F000F0u, 0x54805480u), s16, a1));
+        emit(c, hfma2(and_xor(x * 16u, 0x00F000F0u, 0x54805480u), s.y, a0), hfma2(and_xor(x, 0x00F000F0u, 0x54805480u), s.y, a0),
+             hfma2(and_xor(x8 * 16u, 0x00F000F0u, 0x54805480u), s.y, a1), hfma2(and_xor(x8, 0x00F000F0u, 0x54805480u), s.y, a1));
     }
 }
-template <int U> __device__ __forceinline__ uint32_t ktu_window(const uint32_t* w, int bit) {       // 32 bits of the run from `bit` on
+__device__ __forceinline__ uint32_t ktu_window(const uint32_t* w, int bit) {        // 32 bits of the run from `bit` on
     return (bit & 31) == 0 ? w[bit >> 5] : __funnelshift_r(w[bit >> 5], w[(bit >> 5) + 1], bit & 31);
 }
 // Words of a chunk: elements (0 2) (1 3) (4 6) (5 7).
-template <int U, typename F> __device__ __forceinline__ void ktu_convert_five(const uint32_t (&w)[6], uint32_t s0, uint32_t s1, uint32_t s, F emit) {
-    const uint32_t s8 = hmul2(s, 0x48004800u), c0 = hmul2(s, hset2(-1412.0f)), c1 = hmul2(s, hset2(-404.0f));
+template <typename F> __device__ __forceinline__ void ktu_convert(const KtuRaw<3>& r, const uint4& s, F emit) {
+    const uint32_t w[6] = {r.u[0], r.u[1], r.u[2], r.u[3], r.u[4], 0u};
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-        const uint32_t t = c == 0 ? s0 : c == 1 ? s0 >> 12 : c == 2 ? __funnelshift_r(s0, s1, 24) : s1 >> 4;      // shared codes 4c ..
+        const uint32_t t = c == 0 ? r.s0 : c == 1 ? r.s0 >> 12 : c == 2 ? __funnelshift_r(r.s0, r.s1, 24) : r.s1 >> 4;      // shared codes 4c ..
         const uint32_t ts = halves(t, t * 8192u);                                                  // 0 2 | 1 3 at bits 0, 6
         uint32_t o[4];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const uint32_t x = ktu_window<U>(w, 40 * c + 20 * g), y = halves(x, x * 64u);          // 1 0 | 3 2
-            const uint32_t a = g == 0 ? hfma2(and_xor(ts, 0x00070007u, 0x64046404u), s, c0) : hfma2(and_xor(ts, 0x01C001C0u, 0x4D004D00u), s, c1);
-            o[2 * g] = hfma2(and_xor(y * 32u, 0x03E003E0u, 0x52005200u), s8, a);
-            o[2 * g + 1] = hfma2(and_xor(y, 0x03E003E0u, 0x52005200u), s8, a);
+            const uint32_t x = ktu_window(w, 40 * c + 20 * g), y = halves(x, x * 64u);             // 1 0 | 3 2
+            const uint32_t a = g == 0 ? hfma2(and_xor(ts, 0x00070007u, 0x64046404u), s.x, s.z) : hfma2(and_xor(ts, 0x01C001C0u, 0x4D004D00u), s.x, s.w);
+            o[2 * g] = hfma2(and_xor(y * 32u, 0x03E003E0u, 0x52005200u), s.y, a);
+            o[2 * g + 1] = hfma2(and_xor(y, 0x03E003E0u, 0x52005200u), s.y, a);
         }
         emit(c, o[0], o[1], o[2], o[3]);
     }
 }
-template <int U, typename F> __device__ __forceinline__ void ktu_convert_six(const uint32_t (&w)[7], uint32_t sw, uint32_t s, F emit) {
-    const uint32_t s4 = hmul2(s, 0x44004400u), c0 = hmul2(s, hset2(-1410.0f)), c1 = hmul2(s, hset2(-450.0f));
+template <typename F> __device__ __forceinline__ void ktu_convert(const KtuRaw<2>& r, const uint4& s, F emit) {
+    const uint32_t w[7] = {r.u[0].x, r.u[0].y, r.u[1].x, r.u[1].y, r.u[2].x, r.u[2].y, 0u};
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-        const uint32_t t = sw >> (8 * c), ts = halves(t, t * 16384u);                              // 0 2 | 1 3 at bits 0, 4
+        const uint32_t t = r.s >> (8 * c), ts = halves(t, t * 16384u);                             // 0 2 | 1 3 at bits 0, 4
         uint32_t o[4];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const uint32_t x = ktu_window<U>(w, 48 * c + 24 * g), y = halves(x, x * 16u);          // 1 0 | 3 2
-            const uint32_t a = g == 0 ? hfma2(and_xor(ts, 0x00030003u, 0x64026402u), s, c0) : hfma2(and_xor(ts, 0x00300030u, 0x54205420u), s, c1);
-            o[2 * g] = hfma2(and_xor(y * 16u, 0x03F003F0u, 0x56005600u), s4, a);
-            o[2 * g + 1] = hfma2(and_xor(y >> 2, 0x03F003F0u, 0x56005600u), s4, a);
+            const uint32_t x = ktu_window(w, 48 * c + 24 * g), y = halves(x, x * 16u);             // 1 0 | 3 2
+            const uint32_t a = g == 0 ? hfma2(and_xor(ts, 0x00030003u, 0x64026402u), s.x, s.z) : hfma2(and_xor(ts, 0x00300030u, 0x54205420u), s.x, s.w);
+            o[2 * g] = hfma2(and_xor(y * 16u, 0x03F003F0u, 0x56005600u), s.y, a);
+            o[2 * g + 1] = hfma2(and_xor(y >> 2, 0x03F003F0u, 0x56005600u), s.y, a);
         }
         emit(c, o[0], o[1], o[2], o[3]);
-    }
-}
-template <int U, typename F> __device__ __forceinline__ void ktu_convert(const KtuRaw<U>& r, uint32_t s, F emit) {
-    if constexpr (U == 4) {
-        ktu_convert_nibbles<U>(r, s, emit);
-    } else if constexpr (U == 3) {
-        const uint32_t w[6] = {r.u[0], r.u[1], r.u[2], r.u[3], r.u[4], 0u};
-        ktu_convert_five<U>(w, r.s0, r.s1, s, emit);
-    } else {
-        const uint32_t w[7] = {r.u[0].x, r.u[0].y, r.u[1].x, r.u[1].y, r.u[2].x, r.u[2].y, 0u};
-        ktu_convert_six<U>(w, r.s, s, emit);
     }
 }
 // Where element e of a row is among the operands, and back.
@@ -340,6 +334,15 @@ __device__ __forceinline__ bool ktu_vote(int id, int threads, bool v) {
 }
 __device__ __forceinline__ void ktu_bar(int id, int threads) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+// The rest of a wait that did not succeed at once (a try sleeps for about two microseconds).
+__device__ __forceinline__ void ktu_wait_slow(uint32_t bar, uint32_t parity, uint32_t max_polls, volatile int* abort) {
+    for (uint32_t i = 0; i < max_polls; ++i) {
+        if (*abort || mbar_try_wait(bar, parity)) return;
+        if (i >= MBAR_FAST_POLLS) __nanosleep(128);
+    }
+    *abort = 1;
+}
+
 // Column sums over the 32 lanes: on return v[0] of lane c holds column c (N = 32), c % N below.
 template <int N> __device__ __forceinline__ void ktu_column_sums(float (&v)[N], int lane) {
 #pragma unroll
@@ -360,12 +363,13 @@ struct __align__(16) KtuShared {
     uint64_t sempty[2], vempty[2], pempty[2], done;                           // read
     uint32_t tmem;
     int seq;
-    long long seq_tile, red[2 * KTU_ALL_WARPS];
+    long long seq_tile, red[2 * 28];
     volatile int abort;
     int wide[8];                                                  // tile's values (and probabilities) are bf16
     uint64_t mask[KT_MAX_T];
     float qf[4][KTU_ROWS], qscale[4];                             // score factors 2^x of the query rows; of all rows where they are the same
-    int same[4], qtop[KTU_WARPS], qlow[KTU_WARPS];
+    int same[4], qtop[KTU_DEC_WARPS], qlow[KTU_DEC_WARPS];
+    uint4 scales[32];                                             // of 2^d, d = 4 - i
     float ck[4][KTU_KEYS];                                        // score factors of the keys
     float4 ref4[KTU_ROWS / 4];                                    // per row 7 - m (+inf: nothing seen yet; NaN: not a number)
     float f[KTU_ROWS];                                            // per row the score factor, where they differ
@@ -373,23 +377,24 @@ struct __align__(16) KtuShared {
 };
 
 template <int U, int NR>
-__global__ void __launch_bounds__(KTU_THREADS, 1)
+__global__ void __launch_bounds__(ktu_threads(NR), 1)
 kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32) {
     chain_wait();
-    constexpr int NC = NR / 2;                                    // columns (query rows) of a thread in the softmax
+    constexpr int SW = ktu_soft_warps(NR), NC = NR / (SW / 4);    // softmax warps; columns (query rows) of a thread in the softmax
+    constexpr int WARP_MMA = KTU_DEC_WARPS + SW, WARP_COPY = WARP_MMA + 1, WARP_SCOUT = WARP_MMA + 2, WARPS = WARP_MMA + 4;
     extern __shared__ uint8_t ktu_smem_raw[];
     __shared__ KtuShared sh;
     const uint32_t sbase = (smem_u32(ktu_smem_raw) + 1023u) & ~1023u;
     uint8_t* const smem = ktu_smem_raw + (sbase - smem_u32(ktu_smem_raw));
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int role = warp / KTU_WARPS, quad = warp & 3, half = warp >> 2 & 1;      // role 0: decode (half: team), 1: softmax, 2: the single warps
+    const int quad = warp & 3, half = warp >> 2 & 1;              // decode: which blocks; softmax: which rows
     const int key = quad * 32 + lane;                             // this thread's key of a tile
     const int G = a.Hq / a.Hkv, R = a.T * G, per_seq = a.Hkv * groups;
 
     // ---- this thread block's run of tiles, and where it begins ----
     int64_t skip, total;
-    ktu_sums<KTU_ALL_WARPS>(a, B, 0, sh.red, &skip, &total);
+    ktu_sums<WARPS>(a, B, 0, sh.red, &skip, &total);
     total *= per_seq;
     const int C = (int)min((int64_t)gridDim.x, total);            // no run is empty
     if ((int)blockIdx.x >= C) return;
@@ -410,23 +415,24 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             if (base > g0) break;
         }
     }
-    if (warp == KTU_WARP_MMA) {
+    if (tid < 32) sh.scales[tid] = ktu_scales<U>(4 - tid);
+    if (warp == WARP_MMA) {
         tmem_alloc(smem_u32(&sh.tmem), KTU_COLS);
         tmem_relinquish();
     }
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(smem_u32(&sh.rfull[i]), 1);
-            mbar_init(smem_u32(&sh.rempty[i]), 4);
+            mbar_init(smem_u32(&sh.rempty[i]), KTU_DEC_WARPS / 2);
             mbar_init(smem_u32(&sh.ready[i]), 1);
-            mbar_init(smem_u32(&sh.kfull[i]), 4);
-            mbar_init(smem_u32(&sh.qfull[i]), KTU_WARPS);
+            mbar_init(smem_u32(&sh.kfull[i]), KTU_DEC_WARPS / 2);
+            mbar_init(smem_u32(&sh.qfull[i]), KTU_DEC_WARPS);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&sh.vfull[i]), 4);
+            mbar_init(smem_u32(&sh.vfull[i]), KTU_DEC_WARPS / 2);
             mbar_init(smem_u32(&sh.sfull[i]), 1);
-            mbar_init(smem_u32(&sh.pfull[i]), KTU_WARPS);
-            mbar_init(smem_u32(&sh.sempty[i]), KTU_WARPS);
+            mbar_init(smem_u32(&sh.pfull[i]), SW);
+            mbar_init(smem_u32(&sh.sempty[i]), SW);
             mbar_init(smem_u32(&sh.vempty[i]), 1);
             mbar_init(smem_u32(&sh.pempty[i]), 1);
         }
@@ -449,39 +455,37 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     const KtuCursor start = cur;
 
     constexpr int UB = ktu_ub(U), SB = ktu_sb(U), NST = ktu_stages(U);
-    constexpr int K_SH = 4 * KTU_KEYS * UB, K_SC = K_SH + 4 * KTU_KEYS * SB, V_UP = K_SC + 4 * KTU_KEYS, V_SH = V_UP + K_SH, V_SC = V_UP + K_SC;
+    constexpr int K_SH = 4 * KTU_KEYS * UB, K_SC = K_SH + 4 * KTU_KEYS * SB, V_UP = K_SC + 4 * KTU_KEYS, V_SC = V_UP + K_SC;
     const uint32_t ring = sbase + KTU_Q + NR * 256;               // stages: upper, shared codes and exponents of the keys, of the values
     const uint32_t vrow = (sbase + KTU_V + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;      // with the swizzle of chunk 0
 
-    // A bounded wait of the whole warp; false: it ran out, here or elsewhere.  A warp whose wait failed waits no more but goes on through
-    // the motions, since others of its role meet it at the named barriers; the outputs are marked in the end.
+    // A bounded wait of the whole warp.  Where one runs out, it sets sh.abort: from then on no wait waits any more and all roles go on
+    // through the motions to the end -- they meet at named barriers, so none may leave early --; the outputs are marked then.
     auto wait = [&](const uint64_t& bar, uint32_t phase) {
-        bool done = mbar_try_wait(smem_u32(&bar), phase & 1u);
-        for (uint32_t i = 0; !done && i < a.max_polls && !sh.abort; ++i) {
-            done = mbar_try_wait(smem_u32(&bar), phase & 1u);
-            if (i >= MBAR_FAST_POLLS) __nanosleep(128);
-        }
-        if (!done) sh.abort = 1;
-        return __all_sync(0xffffffffu, done) != 0;
+        if (!mbar_try_wait(smem_u32(&bar), phase & 1u)) ktu_wait_slow(smem_u32(&bar), phase & 1u, a.max_polls, &sh.abort);
+        __syncwarp();
     };
     auto arrive = [&](const uint64_t& bar) {
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar));
     };
 
-    if (role == 0) {
+    if (warp < KTU_DEC_WARPS) {
         // ================================ decode ================================
+        if (SW == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        const int team = warp >> 3;
+        const uint32_t tab = smem_u32(sh.scales);
         int seg = -1;
         uint32_t n_slot = 0, r_phase = 0;                         // the tile's slot of the ring
-        bool ok = true;
 #pragma unroll 1
         for (int j = 0; j < n_run; ++j) {
             if (j == 0 || cur.t == 0) {
                 // ---- a new item: its queries, rotated, scaled by a power of two per row, fp16, K-major with 128-byte swizzle ----
                 ++seg;
-                if (j > 0) ok = ok && wait(sh.sfull[(j - 1) & 1], (uint32_t)(j - 1) >> 1);      // the last item's products have read theirs
+                if (j > 0) wait(sh.sfull[(j - 1) & 1], (uint32_t)(j - 1) >> 1);      // the last item's products have read theirs
                 const int hk = cur.hk, r0 = cur.grp * NR, rows = min(NR, R - r0);
-                constexpr int QR = NR / KTU_WARPS;                // rows of a warp
+                constexpr int QR = NR / KTU_DEC_WARPS;            // rows of a warp
                 float v[QR][4];
                 int top = -128, low = 127;                        // exponents of the rows that are numbers and not zero
                 uint32_t bad = 0u;                                // rows with an infinity or a NaN: NaN, the others are not touched
@@ -514,9 +518,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     else if (ax) { top = max(top, E[k]); low = min(low, E[k]); }
                 }
                 if (lane == 0) { sh.qtop[warp] = top; sh.qlow[warp] = low; }
-                ktu_bar(1, KTU_WARPS * 32);
-#pragma unroll
-                for (int w = 0; w < KTU_WARPS; ++w) { top = max(top, sh.qtop[w]); low = min(low, sh.qlow[w]); }
+                ktu_bar(1, KTU_DEC_WARPS * 32);
+#pragma unroll 1
+                for (int w = 0; w < KTU_DEC_WARPS; ++w) { top = max(top, sh.qtop[w]); low = min(low, sh.qlow[w]); }
                 // largest element to [1024, 2048): of all rows where the smallest row still has its eleven digits then, else of each row
                 const bool same = low >= top - 12;
 #pragma unroll
@@ -538,66 +542,72 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             const uint32_t slot = n_slot, phase = r_phase;
             if (++n_slot == NST) { n_slot = 0; r_phase ^= 1u; }
             cur.next(a, groups, B);
-            if ((j & 1) != half) continue;                        // the other team's tile
-            ok = ok && wait(sh.rfull[slot], phase);
-            ok = ok && wait(sh.ready[slot], phase);
+            if ((j & 1) != team) continue;                        // the other team's tile
+            wait(sh.rfull[slot], phase);
+            wait(sh.ready[slot], phase);
             const uint32_t st = ring + slot * ktu_stage_bytes(U);
             // ---- keys to tensor memory, once the product before the last has read the buffer ----
-            const uint32_t es = lds_s8<K_SC>(st + key) & 0xFF | (lds_s8<K_SC + KTU_KEYS>(st + key) & 0xFF) << 8 |
-                                (lds_s8<K_SC + 2 * KTU_KEYS>(st + key) & 0xFF) << 16 | lds_s8<K_SC + 3 * KTU_KEYS>(st + key) << 24;
-            const int emax = max(max((int)(es << 24) >> 24, (int)(es << 16) >> 24), max((int)(es << 8) >> 24, (int)es >> 24));
-            sh.ck[j & 3][key] = a.sm_scale_log2 * exp2_int(emax);
-            if (j > 1) ok = ok && wait(sh.sfull[half], (uint32_t)(j - 2) >> 1);
+            const uint32_t se = st + key;
+            const int e0 = lds_s8<0>(se + K_SC + 2 * half * KTU_KEYS), e1 = lds_s8<KTU_KEYS>(se + K_SC + 2 * half * KTU_KEYS);
+            const int emax = max(max(e0, e1), max((int)lds_s8<0>(se + K_SC + (2 - 2 * half) * KTU_KEYS), (int)lds_s8<KTU_KEYS>(se + K_SC + (2 - 2 * half) * KTU_KEYS)));
+            if (half == 0) sh.ck[j & 3][key] = a.sm_scale_log2 * exp2_int(emax);
+            const bool wide = sh.wide[j & 7] != 0;
+            if (j > 1) wait(sh.sfull[team], (uint32_t)(j - 2) >> 1);
             tc_fence_after();
-            // (block loops stay rolled: the roles' code shares an instruction cache)
+            const uint32_t row = vrow + team * 32768 + half * 16384;
+            // This thread's two blocks of the key, then of the value.  (One rolled loop for all: the roles share an instruction cache, and with
+            // the blocks unrolled this kernel took a third longer.)
+            uint32_t up = st + (2 * half * KTU_KEYS + key) * UB, shd = st + K_SH + (2 * half * KTU_KEYS + key) * SB;
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
                 KtuRaw<U> raw;
-                ktu_load(raw, st + i * KTU_KEYS * UB + key * UB, st + K_SH + i * KTU_KEYS * SB + key * SB);
+                ktu_load(raw, up, shd);
+                up += i == 1 ? V_UP - KTU_KEYS * UB : KTU_KEYS * UB;
+                shd += i == 1 ? V_UP - KTU_KEYS * SB : KTU_KEYS * SB;
+                int d = (i == 0 ? e0 : e1) - emax;
+                if (i >= 2) {
+                    if (i == 2) {
+                        ktu_st_wait();
+                        tc_fence_before();
+                        arrive(sh.kfull[j & 3]);
+                        // the product before the last has read the values' buffer
+                        if (j > 1) wait(sh.vempty[team], (uint32_t)(j - 2) >> 1);
+                    }
+                    // (in bf16: the codes here, their exponent below; out of range otherwise: zeros, or a key that no row attends)
+                    d = wide ? 0 : min(lds_s8<0>(se + V_SC + (2 * half + i - 2) * KTU_KEYS), 4 - KTU_V_BITS) + KTU_V_BITS;
+                }
+                const uint4 sc = lds128(tab + (4 - max(d, -27)) * 16);
                 uint32_t w[16];
-                ktu_convert<U>(raw, ktu_pow2_h2(((int)(es << (24 - 8 * i)) >> 24) - emax), [&](int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+                ktu_convert(raw, sc, [&](int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
                     w[4 * c] = w0; w[4 * c + 1] = w1; w[4 * c + 2] = w2; w[4 * c + 3] = w3;
                 });
-                ktu_st16(tlane + KTU_COL_K + half * 64 + i * 16, w);
-            }
-            ktu_st_wait();
-            tc_fence_before();
-            arrive(sh.kfull[j & 3]);
-            // ---- values to shared memory, once the product before the last has read them ----
-            if (j > 1) ok = ok && wait(sh.vempty[half], (uint32_t)(j - 2) >> 1);
-            const uint32_t row = vrow + half * 32768;
-            const bool wide = sh.wide[j & 7] != 0;
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-                KtuRaw<U> raw;
-                ktu_load(raw, st + V_UP + i * KTU_KEYS * UB + key * UB, st + V_SH + i * KTU_KEYS * SB + key * SB);
-                const int ve = lds_s8<V_SC>(st + i * KTU_KEYS + key);
-                const uint32_t at = row + (i >> 1) * 16384;
-                if (!wide) {
-                    // (out of range: zeros, or a key that no row attends)
-                    ktu_convert<U>(raw, ktu_pow2_h2(min(max(ve, -100), 4 - KTU_V_BITS) + KTU_V_BITS),
-                                   [&](int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) { sts128(at ^ ((i & 1) * 4 + c) << 4, w0, w1, w2, w3); });
-                } else {
-                    const float sc = exp2_int(max(-126, min(116, ve + KTU_V_BITS)));
-                    const auto bf = [&](uint32_t w) {                         // eight digits: exact
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-                        return prmt(__float_as_uint(f.x * sc), __float_as_uint(f.y * sc), 0x7632u);
-                    };
-                    ktu_convert<U>(raw, 0x3C003C00u, [&](int c, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
-                        sts128(at ^ ((i & 1) * 4 + c) << 4, bf(w0), bf(w1), bf(w2), bf(w3));
-                    });
+                if (i < 2) {
+                    ktu_st16(tlane + KTU_COL_K + team * 64 + half * 32 + i * 16, w);
+                    continue;
                 }
+                if (wide) {
+                    const float f = exp2_int(max(-126, min(116, lds_s8<0>(se + V_SC + (2 * half + i - 2) * KTU_KEYS) + KTU_V_BITS)));
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {                            // eight digits: exact
+                        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[c]));
+                        w[c] = prmt(__float_as_uint(q.x * f), __float_as_uint(q.y * f), 0x7632u);
+                    }
+                }
+                const uint32_t to = row ^ (i & 1) << 6;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sts128(to ^ c << 4, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
             }
             arrive(sh.rempty[slot]);
             fence_async_smem();
-            arrive(sh.vfull[half]);
+            arrive(sh.vfull[team]);
         }
-    } else if (role == 1) {
+    } else if (warp < WARP_MMA) {
         // ================================ softmax ================================
+        if (SW == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         const uint32_t prow = (sbase + KTU_P + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;
-        const int stid = tid - KTU_WARPS * 32, htid = stid & 127;             // thread of the role, of its half
+        const int stid = tid - KTU_DEC_WARPS * 32, htid = stid & 127;             // thread of the role, of its half
         int seg = -1, n_seg = 0;
-        bool ok = true;
         bool same = true;                                         // the item's query rows have one score factor
         float qscale = 1.0f;
         uint64_t l[NC / 2];                                       // sums of pairs of rows over this thread's keys
@@ -607,8 +617,8 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             if (j == 0 || cur.t == 0) {
                 ++seg;
                 n_seg = 0;
-                ok = ok && wait(sh.qfull[seg & 3], (uint32_t)seg >> 2);
-                ktu_bar(2, KTU_WARPS * 32);                       // the last item's masks and references are read
+                wait(sh.qfull[seg & 3], (uint32_t)seg >> 2);
+                ktu_bar(2, SW * 32);                       // the last item's masks and references are read
                 if (stid < a.T) sh.mask[stid] = a.mask[cur.b * a.mask_stride + stid];
                 if (stid < NR) {
                     const float f = sh.qf[seg & 3][stid];
@@ -618,13 +628,13 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 }
                 same = sh.same[seg & 3] != 0;
                 qscale = sh.qscale[seg & 3];
-                ktu_bar(2, KTU_WARPS * 32);
+                ktu_bar(2, SW * 32);
 #pragma unroll
                 for (int c = 0; c < NC / 2; ++c) l[c] = 0ull;
             }
             const int jb = cur.t * KTU_KEYS;
             const bool tail = jb + KTU_KEYS > cur.len;            // the tile has nodes of the tree
-            ok = ok && wait(sh.kfull[j & 3], (uint32_t)j >> 2);
+            wait(sh.kfull[j & 3], (uint32_t)j >> 2);
             const float ck = same ? sh.ck[j & 3][key] * qscale : sh.ck[j & 3][key];
             const bool wide = sh.wide[j & 7] != 0;
             uint32_t vis = 0xFFFFFFFFu;                           // which of this thread's rows attend its key
@@ -639,7 +649,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         }
                 }
             }
-            ok = ok && wait(sh.sfull[j & 1], (uint32_t)j >> 1);
+            wait(sh.sfull[j & 1], (uint32_t)j >> 1);
             tc_fence_after();
             const uint32_t scol = tlane + KTU_COL_S + (j & 1) * 64 + half * NC;
             float x[NC];
@@ -661,7 +671,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         if (!(vis >> c & 1)) x[c] = -INFINITY;
             };
             // the product before the last has read this tile's buffer of the probabilities
-            if (j > 1) ok = ok && wait(sh.pempty[j & 1], (uint32_t)(j - 2) >> 1);
+            if (j > 1) wait(sh.pempty[j & 1], (uint32_t)(j - 2) >> 1);
             bool moved = false;
 #pragma unroll 1
             for (;;) {
@@ -672,10 +682,10 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     top = fmaxf(top, x[c]);
                     top1 = fmaxf(top1, x[c + 1]);
                 }
-                if (moved || !ktu_vote(3 + half, KTU_WARPS * 16, n_seg == 0 || fmaxf(top, top1) > KTU_MOVE)) break;
+                if (moved || !ktu_vote(3 + half, 128, n_seg == 0 || fmaxf(top, top1) > KTU_MOVE)) break;
                 moved = true;
                 // ---- references move: rows of this half whose maximum of this tile is beyond theirs ----
-                if (n_seg > 0) ok = ok && wait(sh.pempty[(j - 1) & 1], (uint32_t)(j - 1) >> 1);  // the accumulators are at rest
+                if (n_seg > 0) wait(sh.pempty[(j - 1) & 1], (uint32_t)(j - 1) >> 1);  // the accumulators are at rest
 #pragma unroll 1
                 for (int c = 0; c < NC; c += 8) {
                     float s[8];
@@ -690,7 +700,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         if (lane == 0) sh.part[quad][r] = __int_as_float(mx ^ (mx >> 31 & 0x7FFFFFFF));
                     }
                 }
-                ktu_bar(3 + half, KTU_WARPS * 16);
+                ktu_bar(3 + half, 128);
                 if (htid < NC) {
                     const int r = half * NC + htid;
                     const float mx = fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), m = sh.m[r];
@@ -703,7 +713,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     }
                     sh.alpha[r] = al;
                 }
-                ktu_bar(3 + half, KTU_WARPS * 16);
+                ktu_bar(3 + half, 128);
                 tc_fence_after();
                 if (n_seg > 0) {
 #pragma unroll 1
@@ -763,7 +773,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     ktu_column_sums<NC>(v, lane);
                     if (lane < NC) sh.part[quad][half * NC + lane] = v[0];
                 }
-                ktu_bar(3 + half, KTU_WARPS * 16);
+                ktu_bar(3 + half, 128);
                 if (htid < NC) {
                     const int r = half * NC + htid;
                     const float s = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
@@ -773,8 +783,8 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         part[r * KTU_PART + 129] = s;
                     }
                 }
-                ktu_bar(3 + half, KTU_WARPS * 16);
-                ok = ok && wait(sh.pempty[j & 1], (uint32_t)j >> 1);
+                ktu_bar(3 + half, 128);
+                wait(sh.pempty[j & 1], (uint32_t)j >> 1);
                 tc_fence_after();
                 const int ch = ktu_element<U>(key);                           // accumulator lane = operand place of the channel
 #pragma unroll 1
@@ -800,7 +810,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             }
             cur.next(a, groups, B);
         }
-    } else if (warp == KTU_WARP_MMA) {
+    } else {
+        if (SW == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    }
+    if (warp == WARP_MMA) {
         // ================================ MMAs ================================
         const uint32_t idesc_qk = ktu_idesc(NR, 0, 0), hi = ktu_desc_hi(1024);
         int seg = -1;
@@ -808,10 +822,10 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         auto issue_qk = [&](int j) {
             if (j == 0 || ahead.t == 0) {
                 ++seg;
-                if (!wait(sh.qfull[seg & 3], (uint32_t)seg >> 2)) return false;
+                wait(sh.qfull[seg & 3], (uint32_t)seg >> 2);
             }
-            if (!wait(sh.kfull[j & 3], (uint32_t)j >> 2)) return false;
-            if (j > 1 && !wait(sh.sempty[j & 1], (uint32_t)(j - 2) >> 1)) return false;
+            wait(sh.kfull[j & 3], (uint32_t)j >> 2);
+            if (j > 1) wait(sh.sempty[j & 1], (uint32_t)(j - 2) >> 1);
             tc_fence_after();
             if (elect_lane()) {
 #pragma unroll
@@ -822,14 +836,14 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             }
             __syncwarp();
             ahead.next(a, groups, B);
-            return true;
         };
         bool first = true;                                        // the next product begins a segment: it overwrites the accumulators
-        if (issue_qk(0))
+        issue_qk(0);
 #pragma unroll 1
-            for (int j = 0; j < n_run; ++j) {
-                if (j + 1 < n_run && !issue_qk(j + 1)) break;
-                if (!wait(sh.vfull[j & 1], (uint32_t)j >> 1) || !wait(sh.pfull[j & 1], (uint32_t)j >> 1)) break;
+        for (int j = 0; j < n_run; ++j) {
+                if (j + 1 < n_run) issue_qk(j + 1);
+                wait(sh.vfull[j & 1], (uint32_t)j >> 1);
+                wait(sh.pfull[j & 1], (uint32_t)j >> 1);
                 tc_fence_after();
                 const uint32_t id = ktu_idesc(NR, sh.wide[j & 7] ? 1u : 0u, 1u);
                 if (elect_lane()) {
@@ -850,7 +864,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             mbar_wait_bounded(smem_u32(&sh.done), 0);
         }
         __syncwarp();
-    } else if (warp == KTU_WARP_COPY) {
+    } else if (warp == WARP_COPY) {
         // ================================ copies ================================
         // Lane 4 p + i brings plane p (keys: upper, shared, exponents; values: the same) of block i.
         const int p = lane >> 2, i = lane & 3, kind = p % 3, per_key = kind == 0 ? UB : kind == 1 ? SB : 1;
@@ -860,7 +874,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         uint32_t slot = 0, phase = 1;                             // passes at once on a fresh barrier
         int issued = 0;
         for (int j = 0; j < n_run; ++j) {
-            if (!wait(sh.rempty[slot], phase)) break;
+            wait(sh.rempty[slot], phase);
             const int n = min(KTU_KEYS, (cur.len + a.T - cur.t * KTU_KEYS + 15) & ~15);            // whole groups of 16 (so is the capacity)
             const int64_t row = (((int64_t)cur.b * a.Hkv + cur.hk) * 4 + i) * a.Lcap + cur.t * KTU_KEYS;
             const uint32_t bar = smem_u32(&sh.rfull[slot]);
@@ -874,11 +888,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         // shared memory is not handed on with a copy in flight
         for (int j = max(0, issued - NST); j < issued; ++j) mbar_wait_bounded(smem_u32(&sh.rfull[j % NST]), (uint32_t)(j / NST) & 1u);
         __syncwarp();
-    } else {
+    } else if (warp == WARP_SCOUT) {
         // ================================ value exponents ================================
         uint32_t slot = 0, phase = 0;
         for (int j = 0; j < n_run; ++j) {
-            if (!wait(sh.rfull[slot], phase)) break;
+            wait(sh.rfull[slot], phase);
             const uint4 v = lds128<V_SC>(ring + slot * ktu_stage_bytes(U) + lane * 16);            // block lane / 8, keys 16 (lane % 8) ..
             const int valid = cur.len + a.T - cur.t * KTU_KEYS - (lane & 7) * 16;
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -899,7 +913,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == KTU_WARP_MMA) tmem_dealloc(tm, KTU_COLS);
+    if (warp == WARP_MMA) tmem_dealloc(tm, KTU_COLS);
     if (sh.abort) {
         // a wait gave up: everything of this run is marked
         if (tid == 0) report_wait_failure(a.sticky, WAIT_FAIL_KV_DECODE);
@@ -909,7 +923,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             if (cur.t == cur.tiles - 1 || j == n_run - 1) {
                 const int r0 = cur.grp * NR, rows = min(NR, R - r0), hk = cur.hk;
                 float* const part = a.partial + ((int64_t)2 * blockIdx.x + (cur.t == n_seg - 1 ? 1 : 0)) * NR * KTU_PART;
-                for (int i = tid; i < rows * 128; i += KTU_THREADS) {
+                for (int i = tid; i < rows * 128; i += WARPS * 32) {
                     const int row = r0 + (i >> 7);
                     const int64_t o = (((int64_t)cur.b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + (i & 127);
                     if (n_seg == cur.tiles) {
