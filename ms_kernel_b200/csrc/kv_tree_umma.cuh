@@ -334,15 +334,6 @@ __device__ __forceinline__ bool ktu_vote(int id, int threads, bool v) {
 }
 __device__ __forceinline__ void ktu_bar(int id, int threads) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// The rest of a wait that did not succeed at once (a try sleeps for about two microseconds).
-__device__ __forceinline__ void ktu_wait_slow(uint32_t bar, uint32_t parity, uint32_t max_polls, volatile int* abort) {
-    for (uint32_t i = 0; i < max_polls; ++i) {
-        if (*abort || mbar_try_wait(bar, parity)) return;
-        if (i >= MBAR_FAST_POLLS) __nanosleep(128);
-    }
-    *abort = 1;
-}
-
 // Column sums over the 32 lanes: on return v[0] of lane c holds column c (N = 32), c % N below.
 template <int N> __device__ __forceinline__ void ktu_column_sums(float (&v)[N], int lane) {
 #pragma unroll
@@ -462,7 +453,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     // A bounded wait of the whole warp.  Where one runs out, it sets sh.abort: from then on no wait waits any more and all roles go on
     // through the motions to the end -- they meet at named barriers, so none may leave early --; the outputs are marked then.
     auto wait = [&](const uint64_t& bar, uint32_t phase) {
-        if (!mbar_try_wait(smem_u32(&bar), phase & 1u)) ktu_wait_slow(smem_u32(&bar), phase & 1u, a.max_polls, &sh.abort);
+        uint32_t left = a.max_polls;                              // (a try sleeps for up to about two microseconds)
+        while (!mbar_try_wait(smem_u32(&bar), phase & 1u))
+            if (sh.abort || --left == 0) { sh.abort = 1; break; }
         __syncwarp();
     };
     auto arrive = [&](const uint64_t& bar) {
@@ -817,6 +810,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     if (warp == WARP_MMA) {
         // ================================ MMAs ================================
         const uint32_t idesc_qk = ktu_idesc(NR, 0, 0), hi = ktu_desc_hi(1024);
+        const uint32_t q_lo = umma_desc_lo(sbase + KTU_Q, 16), v_lo = umma_desc_lo(sbase + KTU_V, 16384), p_lo = umma_desc_lo(sbase + KTU_P, 8192);
         int seg = -1;
         KtuCursor ahead = cur;                                    // of the scores' product, one tile in front
         auto issue_qk = [&](int j) {
@@ -828,10 +822,10 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             if (j > 1) wait(sh.sempty[j & 1], (uint32_t)(j - 2) >> 1);
             tc_fence_after();
             if (elect_lane()) {
-#pragma unroll
+#pragma unroll 1
                 for (int s = 0; s < 8; ++s)
                     ktu_mma_ts(tm + KTU_COL_S + (j & 1) * 64, tm + KTU_COL_K + (j & 1) * 64 + 8 * s,
-                               umma_desc_lo(sbase + KTU_Q + (s >> 2) * (NR * 128) + (s & 3) * 32, 16), hi, idesc_qk, s > 0);
+                               q_lo + (s >> 2) * (NR * 8) + (s & 3) * 2, hi, idesc_qk, s > 0);
                 if (!(a.skip_stage == j && blockIdx.x == 0)) tc_commit(smem_u32(&sh.sfull[j & 1]));
             }
             __syncwarp();
@@ -847,10 +841,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 tc_fence_after();
                 const uint32_t id = ktu_idesc(NR, sh.wide[j & 7] ? 1u : 0u, 1u);
                 if (elect_lane()) {
-#pragma unroll
+#pragma unroll 1
                     for (int s = 0; s < 8; ++s)
-                        ktu_mma_ss(tm + KTU_COL_O, umma_desc_lo(sbase + KTU_V + (j & 1) * 32768 + s * 2048, 16384), hi,
-                                   umma_desc_lo(sbase + KTU_P + (j & 1) * 16384 + s * 2048, 8192), hi, id, !first || s > 0);
+                        ktu_mma_ss(tm + KTU_COL_O, v_lo + (j & 1) * 2048 + s * 128, hi, p_lo + (j & 1) * 1024 + s * 128, hi, id, !first || s > 0);
                     tc_commit(smem_u32(&sh.vempty[j & 1]));
                     tc_commit(smem_u32(&sh.pempty[j & 1]));
                 }
@@ -895,12 +888,13 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             wait(sh.rfull[slot], phase);
             const uint4 v = lds128<V_SC>(ring + slot * ktu_stage_bytes(U) + lane * 16);            // block lane / 8, keys 16 (lane % 8) ..
             const int valid = cur.len + a.T - cur.t * KTU_KEYS - (lane & 7) * 16;
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
             bool far = false;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int e = (int)(w[k >> 2] << (24 - 8 * (k & 3))) >> 24;
-                far = far || (k < valid && e > -100 && (unsigned)(e + 24 + KTU_V_BITS) > 28u);
+            uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k, lo >>= 8, hi >>= 8) {
+                const int e0 = (int8_t)lo, e1 = (int8_t)hi;
+                far = far || (k < valid && e0 > -100 && (unsigned)(e0 + 24 + KTU_V_BITS) > 28u) ||
+                      (k + 8 < valid && e1 > -100 && (unsigned)(e1 + 24 + KTU_V_BITS) > 28u);
             }
             far = __any_sync(0xffffffffu, far);
             if (lane == 0) sh.wide[j & 7] = far;
