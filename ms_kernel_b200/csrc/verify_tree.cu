@@ -10,11 +10,14 @@
 // orders of a sum then part at a border about once in 10^10 draws (in 32 bits once in a few hundred).
 //
 // What bounds it: latency.  Only rows of visited nodes are read -- p (and q) of a node that rejects a child, and of the last one --
-// a megabyte at most per sequence of a row's length 128256.  A cluster of eight thread blocks takes one sequence.  Every block walks
+// a megabyte per pass over a row of 128256.  A cluster of eight thread blocks takes one sequence.  Every block walks
 // the tree by itself on the p(x), q(x) of all candidates, fetched in one round trip; a pass over the vocabulary is shared: a warp
 // sums a piece of neighbours, the sums of all warps go into every block's shared memory, and the sum of the last pass is
 // also the table in which the token is looked up, so the search reads one warp's piece.  The residual is not stored: an
-// element's value after n rejections follows from p, q and the n factors Z.
+// element's value after n rejections follows from p, q and the n factors Z.  The code is kept small: unrolled further, with a loop
+// over the rejections around each element, the kernel spent most of its time fetching instructions (one sequence, 8 nodes, 32000
+// entries, no draft: 27 us, now 8.0 of which 5.2 on the device; 16 sequences, 64 nodes, 128256 entries, up to five
+// rejections in a row: 75 us, now 45).
 #include "msaq_common.cuh"
 #include "sm100_ptx.cuh"
 
@@ -22,7 +25,7 @@ namespace msaq {
 namespace {
 
 constexpr int VF_CLUSTER = 8, VF_WARPS = 16, VF_PIECES = VF_CLUSTER * VF_WARPS, VF_MAX_T = 64;
-constexpr int VF_UNROLL = 4;                 // pieces of 128 elements that a warp has in flight
+constexpr int VF_UNROLL = 4;                 // runs of 128 elements that a warp has in flight
 
 struct VerifyArgs {
     const void* p;                           // target probabilities [B][T][V], strides in elements
@@ -76,17 +79,40 @@ struct Residual {
     int n;
 };
 
-template <bool DRAFT>
-__device__ __forceinline__ double vf_residual(const Residual& r, float p, float q, int i) {
-    double v = (double)vf_clean(p);
-    if (DRAFT && r.n) {
-        const double qc = (double)vf_clean(q);
-        for (int k = 0; k < r.n; ++k) v = fmax(__dsub_rn(v, __dmul_rn(r.Z[k], qc)), 0.0);
+// Elements i + 128 k .. i + 128 k + 3 of the row behind `res`, k < N, those at or beyond i1 as 0.
+template <int N, typename P, bool DRAFT>
+__device__ __forceinline__ void vf_residual(const VerifyArgs& a, const Residual& res, const P* prow, const P* qrow, int i, int i1,
+                                            double (&r)[4 * N]) {
+    float p[N][4], q[N][4];
+#pragma unroll
+    for (int k = 0; k < N; ++k) vf_four(prow, i + 128 * k, i1, a.p_vec, p[k]);
+    if (DRAFT && res.n)
+#pragma unroll
+        for (int k = 0; k < N; ++k) vf_four(qrow, i + 128 * k, i1, a.q_vec, q[k]);
+#pragma unroll
+    for (int e = 0; e < 4 * N; ++e) r[e] = (double)vf_clean(p[e >> 2][e & 3]);
+    if (DRAFT && res.n) {
+        double d[4 * N];
+#pragma unroll
+        for (int e = 0; e < 4 * N; ++e) d[e] = (double)vf_clean(q[e >> 2][e & 3]);
+#pragma unroll 1
+        for (int n = 0; n < res.n; ++n) {
+            const double z = res.Z[n];
+#pragma unroll
+            for (int e = 0; e < 4 * N; ++e) {
+                r[e] = __dsub_rn(r[e], __dmul_rn(z, d[e]));
+                if (!(r[e] > 0.0)) r[e] = 0.0;
+            }
+        }
     }
     if (!DRAFT)
-        for (int k = 0; k < r.n; ++k)
-            if (r.gone[k] == i) v = 0.0;
-    return v;
+#pragma unroll 1
+        for (int n = 0; n < res.n; ++n) {
+            const int at = res.gone[n] - i;
+#pragma unroll
+            for (int e = 0; e < 4 * N; ++e)
+                if (at == 128 * (e >> 2) + (e & 3)) r[e] = 0.0;
+        }
 }
 
 template <typename P, bool DRAFT>
@@ -163,18 +189,12 @@ verify_tree_kernel(const VerifyArgs a) {
         for (;;) {
             const int i0 = (int)(rank * VF_WARPS + warp) * a.piece, i1 = min(i0 + a.piece, a.V);
             double s = 0.0;
-            for (int i = i0; i < i1; i += 128 * VF_UNROLL) {
-                float p[VF_UNROLL][4], q[VF_UNROLL][4];
+#pragma unroll 1
+            for (int i = i0 + 4 * lane; i < i1; i += 128 * VF_UNROLL) {
+                double r[4 * VF_UNROLL];
+                vf_residual<VF_UNROLL, P, DRAFT>(a, res, prow, qrow, i, i1, r);
 #pragma unroll
-                for (int k = 0; k < VF_UNROLL; ++k) {
-                    const int at = i + 128 * k + 4 * lane;
-                    vf_four(prow, at, i1, a.p_vec, p[k]);
-                    if (DRAFT && res.n) vf_four(qrow, at, i1, a.q_vec, q[k]);
-                }
-#pragma unroll
-                for (int k = 0; k < VF_UNROLL; ++k)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s += vf_residual<DRAFT>(res, p[k][e], q[k][e], i + 128 * k + 4 * lane + e);
+                for (int k = 0; k < 4 * VF_UNROLL; k += 4) s += (r[k] + r[k + 1]) + (r[k + 2] + r[k + 3]);
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -235,43 +255,29 @@ verify_tree_kernel(const VerifyArgs a) {
                 if (owner && piece >= 0) {
                     const int i0 = piece * a.piece, i1 = min(i0 + a.piece, a.V);
                     int lastpos = -1;
-                    for (int i = i0; i < i1 && token < 0; i += 128 * 2 * VF_UNROLL) {
-                        float p[2 * VF_UNROLL][4], q[2 * VF_UNROLL][4];
+#pragma unroll 1
+                    for (int i = i0 + 4 * lane; i - 4 * lane < i1 && token < 0; i += 128) {
+                        double r[4];
+                        vf_residual<1, P, DRAFT>(a, res, prow, qrow, i, i1, r);
+                        double incl = (r[0] + r[1]) + (r[2] + r[3]);
+                        int pos = -1, found = -1;
 #pragma unroll
-                        for (int k = 0; k < 2 * VF_UNROLL; ++k) {
-                            const int at = i + 128 * k + 4 * lane;
-                            vf_four(prow, at, i1, a.p_vec, p[k]);
-                            if (DRAFT && res.n) vf_four(qrow, at, i1, a.q_vec, q[k]);
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const double t = __shfl_up_sync(0xffffffffu, incl, o);
+                            if (lane >= o) incl += t;
                         }
+                        double c = __shfl_up_sync(0xffffffffu, incl, 1);
+                        c = cum + (lane ? c : 0.0);
 #pragma unroll
-                        for (int k = 0; k < 2 * VF_UNROLL; ++k) {
-                            const int at = i + 128 * k + 4 * lane;
-                            double r[4], incl = 0.0;
-                            int pos = -1;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                r[e] = vf_residual<DRAFT>(res, p[k][e], q[k][e], at + e);
-                                incl += r[e];
-                                if (r[e] > 0.0) pos = at + e;
-                            }
-#pragma unroll
-                            for (int o = 1; o < 32; o <<= 1) {
-                                const double t = __shfl_up_sync(0xffffffffu, incl, o);
-                                if (lane >= o) incl += t;
-                            }
-                            double c = __shfl_up_sync(0xffffffffu, incl, 1);
-                            c = cum + (lane ? c : 0.0);
-                            int found = -1;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                c += r[e];
-                                if (found < 0 && r[e] > 0.0 && c > limit) found = at + e;
-                            }
-                            const unsigned f = __ballot_sync(0xffffffffu, found >= 0), l = __ballot_sync(0xffffffffu, pos >= 0);
-                            if (token < 0 && f) token = __shfl_sync(0xffffffffu, found, __ffs(f) - 1);
-                            if (l) lastpos = __shfl_sync(0xffffffffu, pos, 31 - __clz(l));
-                            cum += __shfl_sync(0xffffffffu, incl, 31);
+                        for (int e = 0; e < 4; ++e) {
+                            c += r[e];
+                            if (r[e] > 0.0) pos = i + e;
+                            if (found < 0 && r[e] > 0.0 && c > limit) found = i + e;
                         }
+                        const unsigned f = __ballot_sync(0xffffffffu, found >= 0), l = __ballot_sync(0xffffffffu, pos >= 0);
+                        if (f) token = __shfl_sync(0xffffffffu, found, __ffs(f) - 1);
+                        if (l) lastpos = __shfl_sync(0xffffffffu, pos, 31 - __clz(l));
+                        cum += __shfl_sync(0xffffffffu, incl, 31);
                     }
                     if (token < 0) token = lastpos;
                 }
