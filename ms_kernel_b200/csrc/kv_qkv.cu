@@ -10,6 +10,8 @@
 //
 // What bounds it: a token moves 2 D (2 Hq + 2 Hkv) + 2 Hkv NB (UB + SB + 1) bytes, so HBM for a prompt and launch and
 // latency for one token.
+#include <algorithm>
+
 #include "kv_quant_row.cuh"
 
 namespace msaq {
@@ -32,8 +34,10 @@ struct QkvArgs {
     double eps;
     int* sticky;
     int B, T, Hq, Hkv, gain_f32;
-    bool wide;                           // x, ld and q_out allow 16-byte accesses
-    int64_t q_blocks, k_blocks;          // thread blocks of the query rows, of the key rows (as many of the value rows)
+    bool wide, rope_wide;                // x, ld and q_out, the tables allow 16-byte accesses
+    int64_t q_blocks, k_blocks;          // lane per element: thread blocks of the query rows, of the key rows (as many of the value rows)
+    int q_heads, kv_heads;               // eight values per lane: heads of a run
+    int kv_chunks, chunks;               // runs of the key heads (as many of the value heads), of all heads of a token
 };
 
 // (mean + eps)^(-1/2) rounded to fp32: one Newton step of third order in 64 bits on the 32-bit estimate (relative error
@@ -41,7 +45,9 @@ struct QkvArgs {
 __device__ __forceinline__ float norm_factor(double ss, int D, double eps) {
     const double m = ss / (double)D + eps;
     if (!(m > 1e-36 && m < 1e36)) return (float)(1.0 / sqrt(m));
-    const double y = (double)rsqrtf((float)m);
+    float y32;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y32) : "f"((float)m));
+    const double y = (double)y32;
     const double e = fma(-m * y, y, 1.0);
     return (float)fma(y * e, fma(0.375, e, 0.5), y);
 }
@@ -50,28 +56,18 @@ __device__ __forceinline__ float gain_at(const void* g, int f32, int i) {
     return f32 ? static_cast<const float*>(g)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i]);
 }
 
-// Where a row goes: its token's sequence, slot and position.  `live` on return: not padding (q), and its slot inside the cache (k, v).
-struct QkvRow {
+// Where a token's rows go: its sequence, slot and position.  `live` on return: not padding (q), and its slot inside the cache (k, v).
+struct QkvToken {
     int64_t token, key, at;
-    int head, b;
+    int b;
     bool live;
 };
 
-__device__ __forceinline__ QkvRow qkv_row(const QkvArgs& a, int64_t row, int heads, bool into_cache, bool report) {
-    QkvRow r;
-    const int64_t rows = (int64_t)a.B * a.T * heads;
-    r.live = row < rows;
-    if (!r.live) row = 0;
-    if (rows <= UINT32_MAX) {
-        const uint32_t tok = (uint32_t)row / (uint32_t)heads;
-        r.head = (int)((uint32_t)row - tok * (uint32_t)heads);
-        r.b = (int)(tok / (uint32_t)a.T);
-        r.token = tok;
-    } else {
-        r.token = row / heads;
-        r.head = (int)(row % heads);
-        r.b = (int)(r.token / a.T);
-    }
+__device__ __forceinline__ QkvToken qkv_token(const QkvArgs& a, int64_t token, bool into_cache, bool report) {
+    QkvToken r;
+    r.live = token < (int64_t)a.B * a.T;
+    r.token = r.live ? token : 0;
+    r.b = (int)((uint32_t)r.token / (uint32_t)a.T);            // B T fits 31 bits
     const int t = (int)(r.token - (int64_t)r.b * a.T);
     if (a.counts && t >= a.counts[r.b]) r.live = false;
     r.key = (a.start_per_seq ? (int64_t)a.start_per_seq[r.b] : a.start) + t;
@@ -90,37 +86,67 @@ __device__ __forceinline__ QkvRow qkv_row(const QkvArgs& a, int64_t row, int hea
     return r;
 }
 
-// The gs = 2 formats: eight values per lane, 8 / EPL rows per warp, nothing through shared memory.
+__device__ __forceinline__ void qkv_floats(const float* p, bool wide, float (&v)[4]) {
+    if (wide) {
+        const float4 t = *reinterpret_cast<const float4*>(p);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    } else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = p[i];
+}
+
+// Eight bf16 as four words.
+__device__ __forceinline__ uint4 qkv_load8(const __nv_bfloat16* p, bool wide) {
+    if (wide) return *reinterpret_cast<const uint4*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__bfloat16_as_ushort(p[2 * i]) | (uint32_t)__bfloat16_as_ushort(p[2 * i + 1]) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The gs = 2 formats: eight values per lane, 4 EPL lanes to a token, 8 / EPL tokens to a warp, nothing through shared memory.  A
+// lane keeps its token's sines and its gains in registers over a run of heads, and the next head's values are on their way while
+// one is worked on; neighbouring tokens fill the sectors of the planes together.  What it spends its time on is instructions (a
+// prompt of 8191 tokens, 32 + 2 x 8 heads: with one head per warp, its index arithmetic and narrow loads of gains and sines, 440
+// per warp and row pair and 96 us; now 59 us, 185 MB at 3.1 TB/s, the schedulers busy four cycles in five).
 template <int EPL, int U>
 __global__ void __launch_bounds__(QKV_WARPS * 32)
 qkv_write8_kernel(const QkvArgs a) {
     chain_release();
     chain_wait();
-    constexpr int D = 32 * EPL, LANES = 4 * EPL, ROWS = 8 / EPL;
+    constexpr int D = 32 * EPL, LANES = 4 * EPL, TOKENS = 8 / EPL * QKV_WARPS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES;
-    int64_t blk = blockIdx.x;
-    const int kind = blk < a.q_blocks ? 0 : blk < a.q_blocks + a.k_blocks ? 1 : 2;
-    blk -= kind == 0 ? 0 : kind == 1 ? a.q_blocks : a.q_blocks + a.k_blocks;
-    const int heads = kind == 0 ? a.Hq : a.Hkv, head0 = kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv;
-    const int64_t row = (blk * QKV_WARPS + warp) * ROWS + lane / LANES;
-    const QkvRow r = qkv_row(a, row, heads, kind != 0, l == 0);
-    const bool in_range = row < (int64_t)a.B * a.T * heads;
-    float v[8];
-    const __nv_bfloat16* src = a.x + r.token * a.ld + (int64_t)(head0 + r.head) * D + l * 8;
-    if (!r.live) {
+    const uint32_t block = blockIdx.x / (uint32_t)a.chunks;
+    int chunk = (int)(blockIdx.x - block * (uint32_t)a.chunks);
+    const int kind = chunk < a.kv_chunks ? 1 : chunk < 2 * a.kv_chunks ? 2 : 0;
+    chunk -= kind == 1 ? 0 : kind == 2 ? a.kv_chunks : 2 * a.kv_chunks;
+    const int per = kind == 0 ? a.q_heads : a.kv_heads, heads = kind == 0 ? a.Hq : a.Hkv;
+    const int h0 = chunk * per, h1 = min(h0 + per, heads);
+    const int64_t token = (int64_t)block * TOKENS + warp * (8 / EPL) + lane / LANES;
+    const QkvToken r = qkv_token(a, token, kind != 0, l == 0 && chunk == 0);
+    const bool in_range = token < (int64_t)a.B * a.T;
+    if (__ballot_sync(0xffffffffu, kind == 0 ? in_range : r.live) == 0u) return;
+
+    const __nv_bfloat16* src = a.x + r.token * a.ld + (int64_t)((kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv) + h0) * D + l * 8;
+    uint4 next = r.live ? qkv_load8(src, a.wide) : make_uint4(0u, 0u, 0u, 0u);
+    const void* gain = kind == 0 ? a.q_gain : kind == 1 ? a.k_gain : nullptr;
+    const bool rope = kind != 2 && a.rope.cos;
+    float g[8], cs[4], sn[4];
+    if (gain)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    } else if (a.wide) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(src);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        for (int i = 0; i < 8; ++i) g[i] = gain_at(gain, a.gain_f32, l * 8 + i);
+    if (rope) {
+        qkv_floats(a.rope.cos + r.at * (D / 2) + l * 4, a.rope_wide, cs);
+        qkv_floats(a.rope.sin + r.at * (D / 2) + l * 4, a.rope_wide, sn);
+    }
+#pragma unroll 1
+    for (int h = h0; h < h1; ++h) {
+        uint32_t w[4] = {next.x, next.y, next.z, next.w};
+        src += D;
+        if (r.live && h + 1 < h1) next = qkv_load8(src, a.wide);
+        float v[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(w[i]); v[2 * i + 1] = bf16_hi(w[i]); }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(src[i]);
-    }
-    if (kind != 2) {
-        const void* gain = kind == 0 ? a.q_gain : a.k_gain;
         if (gain) {
             double ss = 0.0;
 #pragma unroll
@@ -129,27 +155,28 @@ qkv_write8_kernel(const QkvArgs a) {
             for (int m = 1; m < LANES; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
             const float f = norm_factor(ss, D, a.eps);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], f), gain_at(gain, a.gain_f32, l * 8 + i));
+            for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], f), g[i]);
         }
-        if (a.rope.cos) {
-            const int64_t at = r.at * (D / 2) + l * 4;
+        if (gain || rope)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                rope_pair(v[2 * i], v[2 * i + 1], a.rope.cos[at + i], a.rope.sin[at + i], &v[2 * i], &v[2 * i + 1]);
-        } else if (gain) {
+            for (int i = 0; i < 4; ++i) {                         // the pairs of rope_pair(), rounded two at a time
+                float y0 = v[2 * i], y1 = v[2 * i + 1];
+                if (rope) {
+                    y0 = __fsub_rn(__fmul_rn(v[2 * i], cs[i]), __fmul_rn(v[2 * i + 1], sn[i]));
+                    y1 = __fadd_rn(__fmul_rn(v[2 * i], sn[i]), __fmul_rn(v[2 * i + 1], cs[i]));
+                }
+                const __nv_bfloat162 y = __floats2bfloat162_rn(y0, y1);
+                w[i] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+        if (kind != 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(__float2bfloat16_rn(v[i]));
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(w[i]); v[2 * i + 1] = bf16_hi(w[i]); }
+            quantize_values8_warp<EPL, U>(v, kind == 1 ? a.k : a.v, (int64_t)r.b * a.Hkv + h, r.key, a.Lcap, r.live, lane);
+            continue;
         }
-    }
-    if (kind == 0) {
-        if (!in_range) return;
-        __nv_bfloat16* dst = a.q_out + row * D + l * 8;
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(r.live ? v[2 * i] : 0.0f, r.live ? v[2 * i + 1] : 0.0f);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
+        if (!in_range) continue;
+        if (!r.live) w[0] = w[1] = w[2] = w[3] = 0u;              // padding: zeros
+        __nv_bfloat16* dst = a.q_out + (r.token * a.Hq + h) * D + l * 8;
         if (a.wide) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         else
 #pragma unroll
@@ -157,9 +184,7 @@ qkv_write8_kernel(const QkvArgs a) {
                 dst[2 * i] = __ushort_as_bfloat16((unsigned short)(w[i] & 0xFFFFu));
                 dst[2 * i + 1] = __ushort_as_bfloat16((unsigned short)(w[i] >> 16));
             }
-        return;
     }
-    quantize_values8_warp<EPL, U>(v, kind == 1 ? a.k : a.v, (int64_t)r.b * a.Hkv + r.head, r.key, a.Lcap, r.live, lane);
 }
 
 // Every other group size: one warp per row, the lane-per-element quantiser.
@@ -178,14 +203,16 @@ qkv_write_kernel(const QkvArgs a, Fmt f) {
     const int heads = kind == 0 ? a.Hq : a.Hkv, head0 = kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv;
     const int64_t row = blk * QKV_WARPS + warp;
     if (row >= (int64_t)a.B * a.T * heads) return;             // whole warps
-    const QkvRow r = qkv_row(a, row, heads, kind != 0, lane == 0);
+    const int64_t token = row / heads;
+    const int head = (int)(row - token * heads);
+    const QkvToken r = qkv_token(a, token, kind != 0, lane == 0);
     if (!r.live) {
         if (kind == 0)
             for (int i = lane; i < D; i += 32) a.q_out[row * D + i] = __float2bfloat16_rn(0.0f);
         return;
     }
     float v[EPL];
-    const __nv_bfloat16* src = a.x + r.token * a.ld + (int64_t)(head0 + r.head) * D + lane * EPL;
+    const __nv_bfloat16* src = a.x + r.token * a.ld + (int64_t)(head0 + head) * D + lane * EPL;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) v[i] = __bfloat162float(src[i]);
     if (kind != 2) {
@@ -210,15 +237,28 @@ qkv_write_kernel(const QkvArgs a, Fmt f) {
         for (int i = 0; i < EPL; ++i) a.q_out[row * D + lane * EPL + i] = __float2bfloat16_rn(v[i]);
         return;
     }
-    quantize_values_warp<EPL>(v, kind == 1 ? a.k : a.v, (int64_t)r.b * a.Hkv + r.head, r.key, a.Lcap, f, rowbuf[warp], codes[warp], lane);
+    quantize_values_warp<EPL>(v, kind == 1 ? a.k : a.v, (int64_t)r.b * a.Hkv + head, r.key, a.Lcap, f, rowbuf[warp], codes[warp], lane);
 }
 
 template <int EPL>
 int launch_qkv(QkvArgs& a, const Fmt& f, bool rows8, cudaStream_t st) {
-    const int64_t per_block = (int64_t)QKV_WARPS * (rows8 ? 8 / EPL : 1), tokens = (int64_t)a.B * a.T;
-    a.q_blocks = (tokens * a.Hq + per_block - 1) / per_block;
-    a.k_blocks = (tokens * a.Hkv + per_block - 1) / per_block;
-    const int64_t blocks = a.q_blocks + 2 * a.k_blocks;
+    const int64_t tokens = (int64_t)a.B * a.T;
+    int64_t blocks;
+    if (rows8) {
+        // Long runs of heads save instructions, many blocks keep the SMs busy: the longest run that leaves three waves.
+        const int64_t of_tokens = (tokens + QKV_WARPS * (8 / EPL) - 1) / (QKV_WARPS * (8 / EPL));
+        for (a.q_heads = 8;; a.q_heads /= 2) {
+            a.kv_heads = std::max(a.q_heads / 2, 1);
+            a.kv_chunks = (a.Hkv + a.kv_heads - 1) / a.kv_heads;
+            a.chunks = 2 * a.kv_chunks + (a.Hq + a.q_heads - 1) / a.q_heads;
+            blocks = of_tokens * a.chunks;
+            if (a.q_heads == 1 || blocks >= 3 * 148 * 8) break;
+        }
+    } else {
+        a.q_blocks = (tokens * a.Hq + QKV_WARPS - 1) / QKV_WARPS;
+        a.k_blocks = (tokens * a.Hkv + QKV_WARPS - 1) / QKV_WARPS;
+        blocks = a.q_blocks + 2 * a.k_blocks;
+    }
     if (blocks > INT32_MAX) return fail(MSAQ_ERR_ARG, "size exceeds the supported range");
     const dim3 grid((unsigned)blocks), block(QKV_WARPS * 32);
     if (!rows8) launch_chained(qkv_write_kernel<EPL>, grid, block, 0, st, a, f);
@@ -330,7 +370,7 @@ extern "C" int msaq_kv_write_qkv(const void* qkv, int64_t ld, void* q_out, int8_
     }
     if ((reinterpret_cast<uintptr_t>(k_upper) | reinterpret_cast<uintptr_t>(v_upper)) & 3)
         return fail(MSAQ_ERR_ARG, "upper planes must be 4-byte aligned");
-    if (gain_is_f32 && ((reinterpret_cast<uintptr_t>(q_gain) | reinterpret_cast<uintptr_t>(k_gain)) & 3))
+    if ((reinterpret_cast<uintptr_t>(q_gain) | reinterpret_cast<uintptr_t>(k_gain)) & (gain_is_f32 ? 3 : 1))
         return fail(MSAQ_ERR_ARG, "gains must be aligned to their type");
     if (int rc = require_sm100()) return rc;
     QkvArgs a{};
@@ -346,6 +386,7 @@ extern "C" int msaq_kv_write_qkv(const void* qkv, int64_t ld, void* q_out, int8_
     a.sticky = sticky_status();
     a.B = (int)B; a.T = (int)T; a.Hq = (int)H; a.Hkv = (int)Hkv;
     a.wide = !((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 15) && ld % 8 == 0;
+    a.rope_wide = !((reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin)) & 15);
     const bool rows8 = gs == 2 && !((reinterpret_cast<uintptr_t>(k_shared) | reinterpret_cast<uintptr_t>(v_shared)) & 1);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (D) {

@@ -143,12 +143,11 @@ __device__ __forceinline__ void quantize_values8_warp(float (&v)[8], const Quant
                     v[i + h] = a - b;
                 }
 #pragma unroll
-        for (int m = 1; m < LANES; m <<= 1)
+        for (int m = 1; m < LANES; m <<= 1) {
+            const float sign = (lane & m) ? -1.0f : 1.0f;         // (a product with it is exact: one instruction, the same sums)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float other = __shfl_xor_sync(0xffffffffu, v[i], m);
-                v[i] = (lane & m) ? (other - v[i]) : (v[i] + other);
-            }
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], sign, __shfl_xor_sync(0xffffffffu, v[i], m));
+        }
         const float inv = (float)(1.0 / sqrt((double)D));
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= inv;
