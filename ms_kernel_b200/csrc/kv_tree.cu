@@ -12,9 +12,6 @@ struct TreePlan {
     int S, key_tile, groups, rows;
 };
 
-// The tuned kernel: head_dim 128, gs = 2, capacity a multiple of 16, planes on 16-byte boundaries (bulk copies).
-bool umma_eligible(int64_t D, int gs, int64_t Lcap) { return D == 128 && gs == 2 && Lcap % 16 == 0; }
-
 // Rows per thread block by the rows there are; as many runs of the line of tiles as there are SMs, or as
 // there can be tiles.
 TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
@@ -25,6 +22,11 @@ TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk
     p.S = (int)std::min<int64_t>(sm_count(), B * Hkv * p.groups * ((Lk + KTU_KEYS - 1) / KTU_KEYS));
     p.key_tile = KTU_KEYS;
     return p;
+}
+
+// The tuned kernel: head_dim 128, gs = 2, capacity a multiple of 16 (and planes on 16-byte boundaries: bulk copies), tiles counted in 31 bits.
+bool umma_eligible(int64_t D, int gs, int64_t Lcap, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
+    return D == 128 && gs == 2 && Lcap % 16 == 0 && B * Hkv * plan_tree_umma(B, T, H, Hkv, Lk).groups <= INT32_MAX / ((Lk + KTU_KEYS - 1) / KTU_KEYS);
 }
 
 template <int U, int NR>
@@ -132,7 +134,7 @@ extern "C" int msaq_kv_tree_attention(const void* q, const int8_t* ks, const uin
         return fail(MSAQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool tuned = umma_eligible(D, gs, Lcap) &&
+    const bool tuned = umma_eligible(D, gs, Lcap, B, T, H, Hkv, Lk) &&
                        !((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs) | reinterpret_cast<uintptr_t>(ku) | reinterpret_cast<uintptr_t>(kh) | reinterpret_cast<uintptr_t>(vu) |
                           reinterpret_cast<uintptr_t>(vh)) & 15) &&
                        !(reinterpret_cast<uintptr_t>(q) & 7);

@@ -119,11 +119,6 @@ __device__ __forceinline__ uint64_t pack2(float a, float b) {
     return r;
 }
 __device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -268,51 +263,30 @@ template <int U> __host__ __device__ __forceinline__ int ktu_element(int p) {
 }
 
 // ---- the line of tiles -------------------------------------------------------------------------
-// Item (b, hk, group) has tiles_of(b) tiles; items in that order, sequences first.  Of the N tiles thread block c of C <= N takes
-// [c N / C, (c + 1) N / C).
-__device__ __forceinline__ int ktu_tiles(const KvTreeArgs& a, int b) { return (kt_len(a, b) + a.T + KTU_KEYS - 1) / KTU_KEYS; }
-__device__ __forceinline__ int64_t ktu_run(int64_t n, int c, int C) { return n / C * c + n % C * c / C; }        // c n / C without overflow
-// The thread block whose run holds tile g.
-__device__ __forceinline__ int ktu_owner(int64_t n, int64_t g, int C) {
-    int c = (int)min((int64_t)C - 1, (int64_t)((double)g * C / (double)n));
-    while (c > 0 && ktu_run(n, c, C) > g) --c;
-    while (c + 1 < C && ktu_run(n, c + 1, C) <= g) ++c;
-    return c;
-}
-
-// Sum of tiles_of over the sequences in front of `b` and over all, by the whole thread block of W warps; red: 2 W words of shared memory.
-template <int W>
-__device__ __forceinline__ void ktu_sums(const KvTreeArgs& a, int B, int b, long long* red, int64_t* before, int64_t* all) {
-    const int tid = threadIdx.x, warp = tid >> 5;
-    long long s = 0, t = 0;
-    for (int i = tid; i < B; i += W * 32) {
-        const int n = ktu_tiles(a, i);
-        t += n;
-        if (i < b) s += n;
+// Item (b, hk, group) has tiles_of(b) tiles; items in that order, sequences first.  Of the n tiles (below 2^31: kv_tree.cu) thread
+// block c of C <= n takes [c n / C, (c + 1) n / C).
+__device__ __forceinline__ uint32_t ktu_tiles(const KvTreeArgs& a, int len) { return (uint32_t)(len + a.T + KTU_KEYS - 1) / KTU_KEYS; }
+struct KtuLine {
+    uint32_t n, C, q, r;
+    __device__ __forceinline__ KtuLine(uint32_t tiles, uint32_t blocks) : n(tiles), C(min(blocks, tiles)), q(tiles / C), r(tiles % C) {}
+    __device__ __forceinline__ uint32_t run(uint32_t c) const { return q * c + r * c / C; }         // c n / C without overflow
+    // The thread block whose run holds tile g.
+    __device__ __forceinline__ uint32_t owner(uint32_t g) const {
+        uint32_t c = min(C - 1u, (uint32_t)__fdividef((float)g * (float)C, (float)n));              // off by one at most
+        while (c > 0u && run(c) > g) --c;
+        while (c + 1u < C && run(c + 1u) <= g) ++c;
+        return c;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        t += __shfl_xor_sync(0xffffffffu, t, o);
-    }
-    if ((tid & 31) == 0) { red[warp] = s; red[W + warp] = t; }
-    __syncthreads();
-    s = t = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) { s += red[w]; t += red[W + w]; }
-    *before = s;
-    *all = t;
-    __syncthreads();
-}
+};
 
 // A place on the line.
 struct KtuCursor {
     int b, hk, grp, t;                                            // sequence, kv head, row group, tile
     int len, tiles;                                               // of the sequence
-    __device__ __forceinline__ void sequence(const KvTreeArgs& a, int seq) {
+    __device__ __forceinline__ void sequence(const KvTreeArgs& a, int seq, int its_len) {
         b = seq;
-        len = kt_len(a, b);
-        tiles = (len + a.T + KTU_KEYS - 1) / KTU_KEYS;
+        len = its_len;
+        tiles = (int)ktu_tiles(a, len);
     }
     __device__ __forceinline__ void next(const KvTreeArgs& a, int groups, int B) {
         if (++t < tiles) return;
@@ -321,7 +295,7 @@ struct KtuCursor {
         grp = 0;
         if (++hk < a.Hkv) return;
         hk = 0;
-        if (b + 1 < B) sequence(a, b + 1);
+        if (b + 1 < B) sequence(a, b + 1, kt_len(a, b + 1));
     }
 };
 
@@ -353,13 +327,13 @@ struct __align__(16) KtuShared {
     uint64_t kfull[4], vfull[2], sfull[2], pfull[2], qfull[4];                // written: keys, values, scores, probabilities, queries
     uint64_t sempty[2], vempty[2], pempty[2], done;                           // read
     uint32_t tmem;
-    int seq;
-    long long seq_tile, red[2 * 28];
+    int len;                                                      // of the first tile's sequence
     volatile int abort;
     int wide[8];                                                  // tile's values (and probabilities) are bf16
     uint64_t mask[KT_MAX_T];
     float qf[4][KTU_ROWS], qscale[4];                             // score factors 2^x of the query rows; of all rows where they are the same
     int same[4], qtop[KTU_DEC_WARPS], qlow[KTU_DEC_WARPS];
+    int64_t row[KTU_ROWS];                                        // where a row goes: in the output, among the partial results
     uint4 scales[32];                                             // of 2^d, d = 4 - i
     float ck[4][KTU_KEYS];                                        // score factors of the keys
     float4 ref4[KTU_ROWS / 4];                                    // per row 7 - m (+inf: nothing seen yet; NaN: not a number)
@@ -383,29 +357,39 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     const int key = quad * 32 + lane;                             // this thread's key of a tile
     const int G = a.Hq / a.Hkv, R = a.T * G, per_seq = a.Hkv * groups;
 
-    // ---- this thread block's run of tiles, and where it begins ----
-    int64_t skip, total;
-    ktu_sums<WARPS>(a, B, 0, sh.red, &skip, &total);
-    total *= per_seq;
-    const int C = (int)min((int64_t)gridDim.x, total);            // no run is empty
-    if ((int)blockIdx.x >= C) return;
-    const int64_t g0 = ktu_run(total, blockIdx.x, C);
-    const int n_run = (int)(ktu_run(total, blockIdx.x + 1, C) - g0);
-    if (warp == 0) {                                              // sequences in steps of 32
-        long long base = 0;
-        for (int i0 = 0; i0 < B; i0 += 32) {
-            const long long n = i0 + lane < B ? (long long)ktu_tiles(a, i0 + lane) * per_seq : 0;
-            long long upto = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long t = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += t;
-            }
-            if (n && base + upto > g0 && base + upto - n <= g0) { sh.seq = i0 + lane; sh.seq_tile = base + upto - n; }
-            base += __shfl_sync(0xffffffffu, upto, 31);
-            if (base > g0) break;
+    // ---- this thread block's run of tiles, and where it begins: every warp for itself ----
+    int len = lane < B ? kt_len(a, lane) : 0;
+    uint32_t mine = lane < B ? ktu_tiles(a, len) : 0u, all = mine;
+    for (int i = lane + 32; i < B; i += 32) all += ktu_tiles(a, kt_len(a, i));
+    const KtuLine line(__reduce_add_sync(0xffffffffu, all) * (uint32_t)per_seq, gridDim.x);
+    if (blockIdx.x >= line.C) return;                             // no run is empty
+    const uint32_t g0 = line.run(blockIdx.x);
+    const int n_run = (int)(line.run(blockIdx.x + 1) - g0);
+    int seq = 0;
+    uint32_t seq_tile = 0u;                                       // the sequence of tile g0, its first tile
+    for (int i0 = 0; i0 < B; i0 += 32) {
+        if (i0 > 0) {
+            len = i0 + lane < B ? kt_len(a, i0 + lane) : 0;
+            mine = i0 + lane < B ? ktu_tiles(a, len) : 0u;
         }
+        const uint32_t n = mine * (uint32_t)per_seq;
+        uint32_t upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, seq_tile + upto > g0);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            seq = i0 + src;
+            len = __shfl_sync(0xffffffffu, len, src);
+            seq_tile += __shfl_sync(0xffffffffu, upto - n, src);
+            break;
+        }
+        seq_tile += __shfl_sync(0xffffffffu, upto, 31);
     }
+    if (tid == 0) sh.len = len;
     if (tid < 32) sh.scales[tid] = ktu_scales<U>(4 - tid);
     if (warp == WARP_MMA) {
         tmem_alloc(smem_u32(&sh.tmem), KTU_COLS);
@@ -436,12 +420,12 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     tc_fence_after();
     const uint32_t tm = sh.tmem, tlane = tm + ((uint32_t)(quad * 32) << 16);
     KtuCursor cur;
-    cur.sequence(a, sh.seq);
+    cur.sequence(a, seq, sh.len);
     {
-        const int item = (int)((g0 - sh.seq_tile) / cur.tiles);
-        cur.t = (int)(g0 - sh.seq_tile - (int64_t)item * cur.tiles);
-        cur.hk = item / groups;
-        cur.grp = item - cur.hk * groups;
+        const uint32_t item = (g0 - seq_tile) / (uint32_t)cur.tiles;
+        cur.t = (int)(g0 - seq_tile - item * (uint32_t)cur.tiles);
+        cur.hk = (int)(item / (uint32_t)groups);
+        cur.grp = (int)item - cur.hk * groups;
     }
     const KtuCursor start = cur;
 
@@ -512,8 +496,8 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 }
                 if (lane == 0) { sh.qtop[warp] = top; sh.qlow[warp] = low; }
                 ktu_bar(1, KTU_DEC_WARPS * 32);
-#pragma unroll 1
-                for (int w = 0; w < KTU_DEC_WARPS; ++w) { top = max(top, sh.qtop[w]); low = min(low, sh.qlow[w]); }
+                top = __reduce_max_sync(0xffffffffu, sh.qtop[lane % KTU_DEC_WARPS]);
+                low = __reduce_min_sync(0xffffffffu, sh.qlow[lane % KTU_DEC_WARPS]);
                 // largest element to [1024, 2048): of all rows where the smallest row still has its eleven digits then, else of each row
                 const bool same = low >= top - 12;
 #pragma unroll
@@ -688,9 +672,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         const int r = half * NC + c + k;
                         float t = s[k] * ck * (same ? 1.0f : sh.f[r]);
                         if (!(vis >> (c + k) & 1) || t != t) t = -INFINITY;
-                        const int o = __float_as_int(t);                      // in the order of whole numbers
-                        const int mx = __reduce_max_sync(0xffffffffu, o ^ (o >> 31 & 0x7FFFFFFF));
-                        if (lane == 0) sh.part[quad][r] = __int_as_float(mx ^ (mx >> 31 & 0x7FFFFFFF));
+                        float mx;
+                        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(mx) : "f"(t));
+                        if (lane == 0) sh.part[quad][r] = mx;
                     }
                 }
                 ktu_bar(3 + half, 128);
@@ -756,8 +740,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
 
             if (cur.t == cur.tiles - 1 || j == n_run - 1) {
                 // ---- the segment's result ----
+                if (j == n_run - 1) chain_release();              // the merge's blocks may come: they wait for this grid, and want no tensor memory
                 const bool whole = n_seg == cur.tiles;            // finished here; else partial result 2 c (not the item's first) or 2 c + 1
-                float* const part = a.partial + ((int64_t)2 * blockIdx.x + (cur.t == n_seg - 1 ? 1 : 0)) * NR * KTU_PART;
+                const int64_t part = ((int64_t)2 * blockIdx.x + (cur.t == n_seg - 1 ? 1 : 0)) * NR * KTU_PART;
                 const int rows = min(NR, R - r0), hk = cur.hk;
                 {
                     float v[NC];
@@ -771,31 +756,31 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     const int r = half * NC + htid;
                     const float s = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
                     sh.alpha[r] = s == 0.0f ? 0.0f : 1.0f / s;
-                    if (!whole && r < rows) {
-                        part[r * KTU_PART + 128] = sh.m[r];
-                        part[r * KTU_PART + 129] = s;
+                    const int row = r0 + r;
+                    sh.row[r] = whole ? (((int64_t)cur.b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 : part + r * KTU_PART;
+                    if (!whole) {
+                        a.partial[part + r * KTU_PART + 128] = sh.m[r];
+                        a.partial[part + r * KTU_PART + 129] = s;
                     }
                 }
                 ktu_bar(3 + half, 128);
                 wait(sh.pempty[j & 1], (uint32_t)j >> 1);
                 tc_fence_after();
                 const int ch = ktu_element<U>(key);                           // accumulator lane = operand place of the channel
+                constexpr float V_SCALE = 1.0f / (1 << KTU_V_BITS);
 #pragma unroll 1
-                for (int c = 0; c < NC; c += 8) {
+                for (int c = half * NC; c < min(half * NC + NC, rows); c += 8) {
                     float o[8];
-                    ktu_ld8(tlane + KTU_COL_O + half * NC + c, o);
+                    ktu_ld8(tlane + KTU_COL_O + c, o);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const int r = half * NC + c + k;
-                        if (r >= rows) continue;
-                        if (whole) {
-                            const int row = r0 + r;
-                            const float f = sh.alpha[r], v = f == 0.0f ? 0.0f : o[k] * (1.0f / (1 << KTU_V_BITS)) * f;
-                            const int64_t at = (((int64_t)cur.b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + ch;
+                        const int64_t at = sh.row[c + k] + ch;
+                        if (!whole) {
+                            a.partial[at] = o[k] * V_SCALE;
+                        } else if (c + k < rows) {
+                            const float f = sh.alpha[c + k], v = f == 0.0f ? 0.0f : o[k] * V_SCALE * f;
                             out[at] = __float2bfloat16_rn(v);
                             if (out_f32) out_f32[at] = v;
-                        } else {
-                            part[r * KTU_PART + ch] = o[k] * (1.0f / (1 << KTU_V_BITS));
                         }
                     }
                 }
@@ -941,17 +926,26 @@ __global__ void __launch_bounds__(256)
 kv_tree_merge_kernel(const KvTreeArgs a, int B, int groups, int blocks, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32) {
     chain_release();
     chain_wait();
-    __shared__ long long red[16];
+    __shared__ uint32_t red[16];
     const int per_seq = a.Hkv * groups, G = a.Hq / a.Hkv, R = a.T * G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int b = blockIdx.y, item = blockIdx.x / (NR / 8), r = blockIdx.x % (NR / 8) * 8 + warp;
     const int hk = item / groups, row = item % groups * NR + r;
-    int64_t before, total;
-    ktu_sums<8>(a, B, b, red, &before, &total);
-    total *= per_seq;
-    const int C = (int)min((int64_t)blocks, total), tiles = ktu_tiles(a, b);
-    const int64_t g = before * per_seq + (int64_t)item * tiles;
-    const int first = ktu_owner(total, g, C), last = ktu_owner(total, g + tiles - 1, C);
+    uint32_t before = 0u, all = 0u;                               // tiles of the sequences in front, of all
+    for (int i = threadIdx.x; i < B; i += 256) {
+        const uint32_t n = ktu_tiles(a, kt_len(a, i));
+        all += n;
+        if (i < b) before += n;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (lane == 0) { red[warp] = before; red[8 + warp] = all; }
+    __syncthreads();
+    before = __reduce_add_sync(0xffffffffu, lane < 8 ? red[lane] : 0u);
+    all = __reduce_add_sync(0xffffffffu, lane < 8 ? red[8 + lane] : 0u);
+    const KtuLine line(all * (uint32_t)per_seq, (uint32_t)blocks);
+    const uint32_t tiles = ktu_tiles(a, kt_len(a, b)), g = before * (uint32_t)per_seq + (uint32_t)item * tiles;
+    const int first = (int)line.owner(g), last = (int)line.owner(g + tiles - 1u);
     if (first == last || row >= R) return;
     const int n = last - first + 1;
     auto slot = [&](int i) { return a.partial + (((int64_t)2 * (first + i) + (i == 0 ? 1 : 0)) * NR + r) * KTU_PART; };
