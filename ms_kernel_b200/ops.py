@@ -258,6 +258,8 @@ class KVCache:
         slots).  counts int32 [B]: how many of a sequence's T tokens are there; the query rows of the others are 0 and
         their slots stay.  T is any length, one token to a prompt."""
         B, T = int(qkv.shape[0]), int(qkv.shape[1])
+        if B != self.B:
+            raise ValueError("qkv has %d sequences, the cache %d" % (B, self.B))
         start_t, start_i = (None, int(start)) if isinstance(start, int) else (start, 0)
         cos, sin = (None, None) if rope is None else (rope[0], rope[1])
         return _OPS.kv_write_qkv(qkv, *self.k, *self.v, start_t, pos, counts, q_gain, k_gain, cos, sin, B, T, int(Hq), self.Hkv,

@@ -147,6 +147,30 @@ def test_write_norm_of_extreme_rows(rng):
         assert np.array_equal(got.cpu().numpy(), ref)
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,D,u", [(2601, 10, 3, 128, 4), (4321, 10, 3, 128, 4), (7201, 10, 3, 128, 3), (7201, 9, 5, 64, 2), (1999, 40, 9, 256, 4)])
+def test_write_prompt_equals_its_pieces(rng, T, Hq, Hkv, D, u):
+    """A long prompt (several heads in a row per lane, the last run shorter) writes what its pieces of 97 tokens write one by one,
+    to the bit, with two sequences, padding, positions that are not the slots and tables on a 4-byte boundary."""
+    B, Lcap = 2, T + 40
+    qkv = _bf(rng.standard_normal((B, T, (Hq + 2 * Hkv) * D), dtype=np.float32))
+    gains = [_bf(1 + 0.3 * rng.standard_normal(D)) for _ in range(2)]
+    tables = [torch.from_numpy(t).cuda() for t in orc.rope_tables(np.arange(Lcap), D)]
+    moved = [torch.cat([t.new_zeros(1), t.flatten()])[1:].view_as(t) for t in tables]
+    assert moved[0].data_ptr() % 16 == 4
+    start, counts = np.array([3, 17]), np.array([T, T - 111])
+    pos = (np.arange(T)[None] // 2 + start[:, None]).astype(np.int32)
+    a, b = _cache(B, Hkv, D, Lcap, u, 2, fill=0x5A), _cache(B, Hkv, D, Lcap, u, 2, fill=0x5A)
+    q = a.write_qkv(qkv, Hq, _i32(start), tables, *gains, EPS, pos=_i32(pos), counts=_i32(counts))
+    for t in range(0, T, 97):
+        n = min(97, T - t)
+        part = b.write_qkv(qkv[:, t:t + n].contiguous(), Hq, _i32(start + t), moved, *gains, EPS, pos=_i32(pos[:, t:t + n]),
+                           counts=_i32(np.clip(counts - t, 0, n)))
+        assert torch.equal(part, q[:, t:t + n])
+    for x, y in zip((*a.k, *a.v), (*b.k, *b.v)):
+        assert torch.equal(x, y)
+    assert _status() == 0
+
+
 # ------------------------------------------------------------------------------------------------ attend_tree
 def _bound(ref, mag, big, all_v, p_step):
     """Elementwise bound of the output's error, relative steps of half a unit: the result's rounding to bf16 (2^-8 of it); of a

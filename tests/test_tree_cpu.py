@@ -99,6 +99,14 @@ def test_operators_refuse_cpu_tensors():
         cache.attend_tree(torch.zeros(2, 2, 4, 128, dtype=torch.bfloat16), torch.ones(2, dtype=torch.int64), 8)
 
 
+def test_write_qkv_refuses_another_batch_than_the_cache():
+    from ms_kernel_b200 import ops
+    cache = ops.KVCache(3, 2, 128, 32, 4, 2, "cpu")
+    for B in (2, 4):
+        with pytest.raises(ValueError):
+            cache.write_qkv(torch.zeros(B, 1, 8 * 128, dtype=torch.bfloat16), 4, 0)
+
+
 @pytest.mark.parametrize("T", [1, 2, 7, 64])
 def test_tree_mask_against_sets(rng, T):
     from ms_kernel_b200 import ops
