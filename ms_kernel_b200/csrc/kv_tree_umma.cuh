@@ -521,7 +521,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             cur.next(a, groups, B);
             if ((j & 1) != team) continue;                        // the other team's tile
             wait(sh.rfull[slot], phase);
-            wait(sh.ready[slot], phase);
+            wait(sh.ready[slot], phase);                          // (before the keys: the softmax takes kfull for a sign that sh.wide is there)
             const uint32_t st = ring + slot * ktu_stage_bytes(U);
             // ---- keys to tensor memory, once the product before the last has read the buffer ----
             const uint32_t se = st + key;
@@ -949,22 +949,16 @@ kv_tree_merge_kernel(const KvTreeArgs a, int B, int groups, int blocks, __nv_bfl
     if (first == last || row >= R) return;
     const int n = last - first + 1;
     auto slot = [&](int i) { return a.partial + (((int64_t)2 * (first + i) + (i == 0 ? 1 : 0)) * NR + r) * KTU_PART; };
-    float mg = -INFINITY;
+    float mg = -INFINITY, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, den = 0.0f;
     bool bad = false;
-    for (int i = lane; i < n; i += 32) {
-        const float m = slot(i)[128];
-        bad = bad || m != m;
-        mg = fmaxf(mg, m);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mg = fmaxf(mg, __shfl_xor_sync(0xffffffffu, mg, o));
-    bad = __any_sync(0xffffffffu, bad);
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, den = 0.0f;
-    for (int i0 = 0; i0 < n; i0 += 8) {
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 8) {                           // eight results on their way at a time, weights relative to the largest so far
         float4 v[8];
-        float m[8], l[8];
+        float m[8], l[8], top = mg;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
             if (i0 + k >= n) continue;
             const float* p = slot(i0 + k);
             v[k] = *reinterpret_cast<const float4*>(p + 4 * lane);
@@ -973,7 +967,17 @@ kv_tree_merge_kernel(const KvTreeArgs a, int B, int groups, int blocks, __nv_bfl
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            if (i0 + k >= n || (m[k] == -INFINITY && l[k] == 0.0f)) continue;     // a part of which the row attends nothing
+            bad = bad || m[k] != m[k];
+            top = fmaxf(top, m[k]);
+        }
+        const float old = mg == top ? 1.0f : exp2f(mg - top);
+        mg = top;
+        den *= old;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] *= old;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (m[k] == -INFINITY && l[k] == 0.0f) continue;       // a part of which the row attends nothing, or none
             const float w = exp2f(m[k] - mg);
             acc[0] = fmaf(v[k].x, w, acc[0]);
             acc[1] = fmaf(v[k].y, w, acc[1]);
