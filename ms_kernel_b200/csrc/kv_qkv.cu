@@ -245,14 +245,17 @@ int launch_qkv(QkvArgs& a, const Fmt& f, bool rows8, cudaStream_t st) {
     const int64_t tokens = (int64_t)a.B * a.T;
     int64_t blocks;
     if (rows8) {
-        // Long runs of heads save instructions, many blocks keep the SMs busy: the longest run that leaves three waves.
+        // Long runs of heads save instructions, many blocks keep the SMs busy: the longest run (of 8, 4, 2 query heads, half as many
+        // key heads, or 1) that leaves six of seven resident blocks per SM.  Runs of 1 / 2 / 4 / 8 took, 32 + 2 x 8 heads: 128 tokens
+        // 3.7 / 3.4 / 4.2 / 5.4 us, 512 tokens 8.3 / 6.9 / 6.0 / 6.9, 1024 tokens 14.2 / 11.9 / 10.1 / 9.7, 8191 tokens 105 / 86 / 67 /
+        // 58 (16: 57, but 17.1 against 16.5 at 2048).
         const int64_t of_tokens = (tokens + QKV_WARPS * (8 / EPL) - 1) / (QKV_WARPS * (8 / EPL));
         for (a.q_heads = 8;; a.q_heads /= 2) {
             a.kv_heads = std::max(a.q_heads / 2, 1);
             a.kv_chunks = (a.Hkv + a.kv_heads - 1) / a.kv_heads;
             a.chunks = 2 * a.kv_chunks + (a.Hq + a.q_heads - 1) / a.q_heads;
             blocks = of_tokens * a.chunks;
-            if (a.q_heads == 1 || blocks >= 3 * 148 * 8) break;
+            if (a.q_heads == 1 || blocks >= 6LL * sm_count()) break;
         }
     } else {
         a.q_blocks = (tokens * a.Hq + QKV_WARPS - 1) / QKV_WARPS;

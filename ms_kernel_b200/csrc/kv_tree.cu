@@ -12,8 +12,9 @@ struct TreePlan {
     int S, key_tile, groups, rows;
 };
 
-// Rows per thread block by the rows there are; as many runs of the line of tiles as there are SMs, or as
-// there can be tiles.
+// Rows per thread block by the rows there are (4 sequences of 32752 keys, in blocks of 16 / 32 / 64: 16 rows 81 / 88 / 105 us, 32 rows
+// 89 against 106; one of 509 keys, 16 rows: 13.1 / 14.7 / 17.2 us); as many runs of the line of tiles as there are SMs, or as there can
+// be tiles.
 TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
     TreePlan p;
     const int64_t R = T * (H / Hkv);
@@ -25,6 +26,8 @@ TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk
 }
 
 // The tuned kernel: head_dim 128, gs = 2, capacity a multiple of 16 (and planes on 16-byte boundaries: bulk copies), tiles counted in 31 bits.
+// (The generic kernel takes 125 instead of 16.7 us at 8 nodes over 509 keys, 16.3 ms instead of 0.35 for 16 sequences of 16 nodes over up to
+// 32752 keys.)
 bool umma_eligible(int64_t D, int gs, int64_t Lcap, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
     return D == 128 && gs == 2 && Lcap % 16 == 0 && B * Hkv * plan_tree_umma(B, T, H, Hkv, Lk).groups <= INT32_MAX / ((Lk + KTU_KEYS - 1) / KTU_KEYS);
 }

