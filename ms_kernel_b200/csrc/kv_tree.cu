@@ -88,8 +88,9 @@ int launch_tree_generic(const KvTreeArgs& a, const TreePlan& p, int B, cudaStrea
     return check_launch("kv_tree_generic");
 }
 
+// (Lk: key indexes, and the ends of tiles behind the last key, stay within 31 bits.)
 bool tree_sizes_ok(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk, int64_t D) {
-    return B > 0 && B <= 65535 && T > 0 && T <= KT_MAX_T && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 65535 && Lk >= T && Lk <= INT32_MAX &&
+    return B > 0 && B <= 65535 && T > 0 && T <= KT_MAX_T && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 65535 && Lk >= T && Lk <= (1 << 30) &&
            (D == 32 || D == 64 || D == 128 || D == 256) && Hkv * ((T * (H / Hkv) + KTG_ROWS - 1) / KTG_ROWS) <= 65535;
 }
 

@@ -107,6 +107,20 @@ def test_write_qkv_refuses_another_batch_than_the_cache():
             cache.write_qkv(torch.zeros(B, 1, 8 * 128, dtype=torch.bfloat16), 4, 0)
 
 
+def test_tree_attention_refuses_more_keys_than_its_indexes_hold():
+    from ms_kernel_b200 import _lib
+    L, one, most = _lib.lib(), 16, 1 << 30
+
+    def call(Lk):
+        return L.msaq_kv_tree_attention(one, *[one] * 3, *[one] * 3, one, None, None, one, 0, 1, 8, 1, 1, Lk, 32, 1, 4, 2, (1 << 31) - 1, 1, one,
+                                        1 << 40, None)
+
+    assert L.msaq_kv_tree_workspace(1, 8, 1, 1, most, 32) > 65536 and L.msaq_kv_tree_workspace(1, 8, 1, 1, most + 1, 32) == 0
+    assert call(most + 1) == -1
+    if not torch.cuda.is_available():
+        assert call(most) == -5
+
+
 @pytest.mark.parametrize("T", [1, 2, 7, 64])
 def test_tree_mask_against_sets(rng, T):
     from ms_kernel_b200 import ops
