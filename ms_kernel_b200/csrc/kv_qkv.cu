@@ -8,8 +8,8 @@
 // y (in 32 bits one key row in about ten thousand would land on other codes).  The remaining steps are fp32 operations,
 // each rounded by itself.
 //
-// What bounds it: a token moves 2 D (2 Hq + 2 Hkv) + 2 Hkv NB (UB + SB + 1) bytes, so HBM for a prompt and launch and
-// latency for one token.
+// A token moves 2 D (2 Hq + 2 Hkv) + 2 Hkv NB (UB + SB + 1) bytes and 4 D of tables: 185 MB for 8191 tokens of 32 + 2 x 8 heads (28 us).
+// What bounds a prompt are the instructions (59 us: qkv_write8_kernel), one token the call (10 us, 2.6 of them on the device).
 #include <algorithm>
 
 #include "kv_quant_row.cuh"
@@ -287,7 +287,8 @@ struct KeepArgs {
 };
 
 // One warp per (sequence, head, block) of one cache reads every row that moves into registers before it writes one, so a row
-// may go where another one comes from.  Two rows per lane cover the 64 nodes of the largest tree.
+// may go where another one comes from.  Two rows per lane cover the 64 nodes of the largest tree.  Latency: two round trips (path, rows)
+// and the call; 6.5 us, 2.2 of them on the device for one small tree, 4.6 for 64 of 61 nodes.
 __global__ void __launch_bounds__(128)
 keep_kernel(const KeepArgs a) {
     chain_release();
