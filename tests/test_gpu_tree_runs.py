@@ -1,0 +1,170 @@
+"""The tree attention where a thread block walks many tiles of keys, and the verification where a warp walks many pieces of the
+vocabulary: against plain forms in 64 bits on the GPU."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import tree_oracle as tro
+from test_gpu_tree import _bf, _bound, _cache, _check_verify, _i32, _random_parents, _verify_case
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+RAGGED = [5900, 130, 260, 2000, 5, 383, 6000, 1400, 77, 3100]
+
+
+def _fields(plane, width, count):
+    """Bytes [..., n] of a dense little-endian run of two's-complement fields -> float64 [..., count]."""
+    bits = (plane[..., None] >> torch.arange(8, device="cuda", dtype=torch.uint8)) & 1
+    bits = bits.reshape(*plane.shape[:-1], -1)[..., :count * width].reshape(*plane.shape[:-1], count, width)
+    weight = torch.tensor([2.0 ** k for k in range(width - 1)] + [-2.0 ** (width - 1)], dtype=torch.float64, device="cuda")
+    return (bits.double() * weight).sum(-1)
+
+
+def _values(planes, u):
+    """Planes of gs = 2 with 32-blocks [Hkv, 4, L, ...] -> values [Hkv, L, 128] in 64 bits."""
+    e, upper, shared = planes
+    q = _fields(upper, 8 - u, 32) * 2.0 ** u + _fields(shared, u, 16).repeat_interleave(2, -1)
+    x = q * torch.exp2(e.double())[..., None]
+    return x.permute(0, 2, 1, 3).reshape(e.shape[0], e.shape[2], D)
+
+
+def _hadamard():
+    h = torch.ones((1, 1), dtype=torch.float64, device="cuda")
+    while len(h) < D:
+        h = torch.cat((torch.cat((h, h), 1), torch.cat((h, -h), 1)))
+    return h / D ** 0.5
+
+
+def _plain(q, c, lens, seen):
+    """tro.tree_attention, one (sequence, kv head) at a time as matrices."""
+    B, T, Hq, _ = q.shape
+    G, H = Hq // c.Hkv, _hadamard()
+    words = torch.from_numpy(np.stack([tro.mask_words(s) for s in seen])).cuda()
+    sees = ((words[..., None] >> torch.arange(T, device="cuda")) & 1).bool()
+    qd = torch.from_numpy(q).cuda().double()
+    if c.rotate:
+        qd = qd @ H
+    out, mag, all_v = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(3))
+    big = torch.zeros(q.shape[:3], dtype=torch.float64, device="cuda")
+    for b in range(B):
+        n = int(lens[b]) + T
+        K, V = (_values([p[b, :, :, :n] for p in pl], c.u) for pl in (c.k, c.v))
+        ok = torch.cat((torch.ones((T, n - T), dtype=torch.bool, device="cuda"), sees[b]), 1).repeat_interleave(G, 0)
+        none = ~ok.any(1)
+        for h in range(c.Hkv):
+            x = qd[b, :, h * G:(h + 1) * G].reshape(T * G, D)
+            s = (x @ K[h].T / D ** 0.5).masked_fill(~ok, -np.inf)
+            p = torch.softmax(s.masked_fill(none[:, None], 0.0), -1).masked_fill(none[:, None], 0.0)
+            a = (x.abs() @ K[h].abs().T / D ** 0.5).masked_fill(~ok, 0.0).amax(1)
+            put = lambda t, y: t[b, :, h * G:(h + 1) * G].copy_(y.reshape(T, G, *y.shape[1:]))
+            put(out, p @ V[h]), put(mag, p @ V[h].abs()), put(all_v, ok.double() @ V[h].abs()), put(big, a)
+    return [t.cpu().numpy() for t in (out, mag, big, all_v)]
+
+
+def _tiles(lens, T, Hkv, G):
+    """Tiles of 128 keys of all items: row groups of 16, 32 or 64 rows."""
+    R = T * G
+    rows = 16 if R <= 16 else 32 if R <= 32 else 64
+    return sum(-(-(int(n) + T) // 128) for n in lens) * Hkv * -(-R // rows)
+
+
+def _case(rng, B, T, Hq, Hkv, u, lens, edit=None, aim=0.0, scale=1.0, least=4.0):
+    """Fills a cache (keys along one direction per head, `aim` times how far into the context a key is) -> cache, queries, mask, lens,
+    seen.  `least`: tiles per SM that the case has at least."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert _tiles(lens, T, Hkv, Hq // Hkv) >= least * sms
+    Lk = int(max(lens)) + T
+    c = _cache(B, Hkv, D, (Lk + 15) // 16 * 16, u, 2, fill=0x7F)
+    g = torch.Generator(device="cuda").manual_seed(int(rng.integers(1 << 30)))
+    w = torch.randn((1, Hkv, 1, D), generator=g, device="cuda")
+    K, V = (torch.randn((B, Hkv, Lk, D), generator=g, device="cuda") for _ in range(2))
+    K += aim * w * (torch.arange(Lk, device="cuda") / Lk)[:, None]
+    q = torch.randn((B, T, Hkv, Hq // Hkv, D), generator=g, device="cuda") * scale
+    if aim:
+        q += w.reshape(Hkv, 1, D)
+    if edit is not None:
+        edit(K, V)
+    for b in range(B):
+        n = int(lens[b]) + T
+        for X, pl, rot in ((K, c.k, True), (V, c.v, False)):
+            part = [p[b:b + 1].contiguous() for p in pl]
+            torch.ops.msaq.kv_write_into(X[b:b + 1, :, :n].to(torch.bfloat16).contiguous(), *part, Hkv, n, D, 4, 0, c.Lcap, u, 2, rot)
+            for p, s in zip(pl, part):
+                p[b:b + 1] = s
+    seen = [tro.tree_mask(_random_parents(rng, T)) for _ in range(B)]
+    mask = torch.from_numpy(np.stack([tro.mask_words(s) for s in seen])).cuda()
+    q = q.reshape(B, T, Hq, D).to(torch.bfloat16).float().cpu().numpy()
+    return c, q, mask, np.asarray(lens), seen
+
+
+def _check(case, p_step=2.0 ** -11):
+    c, q, mask, lens, seen = case
+    Lk = int(max(lens)) + q.shape[1]
+    got = c.attend_tree(_bf(q), mask, Lk, _i32(lens))
+    again = c.attend_tree(_bf(q), mask, Lk, _i32(lens))
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+    got = got.float().cpu().numpy()
+    assert np.isfinite(got).all()
+    ref, mag, big, all_v = _plain(q, c, lens, seen)
+    err, lim = np.abs(got - ref), _bound(ref, mag, big, all_v, p_step)
+    assert (err <= lim).all(), "worst %.3f of the bound" % (err / lim).max()
+    return got, ref
+
+
+# T and query heads to a kv head: 16, 32, 64 rows, and three groups of 64 of which the last is not full
+ROWS = [(8, 2), (16, 2), (16, 4), (47, 3)]
+
+
+@pytest.mark.parametrize("u", [4, 3, 2])
+@pytest.mark.parametrize("T,G", ROWS)
+def test_runs_of_many_tiles(rng, T, G, u):
+    """Items longer and shorter than a run: ring slots, barriers and buffers are used again and again, queries of several items staged
+    in one run, items finished in it or cut."""
+    _check(_case(rng, 10, T, 8 * G, 8, u, RAGGED))
+
+
+@pytest.mark.parametrize("aim", [1.5, 6.0, -3.0])
+@pytest.mark.parametrize("T,G", ROWS)
+def test_maximum_moves_within_a_run(rng, T, G, aim):
+    """Scores that rise along the context (by 25 to 100 powers of two), or fall: references move while accumulators hold earlier tiles."""
+    _check(_case(rng, 10, T, 8 * G, 8, 4, RAGGED, aim=aim, scale=0.3))
+
+
+@pytest.mark.parametrize("u", [4, 2])
+@pytest.mark.parametrize("T,G", ROWS)
+def test_narrow_and_wide_values_in_a_run(rng, T, G, u):
+    """Tiles whose values leave the range of fp16 between tiles whose values do not."""
+    def edit(K, V):
+        V[:, ::2, 300:310] *= 2.0 ** 12
+        V[:, 1::2, 777] *= 2.0 ** 14
+        V[:, :, 900:1100] *= 2.0 ** -26
+        V[:, :, 2048:2050] *= 2.0 ** -40
+        K[:, :, 512:640] *= 3
+
+    _check(_case(rng, 10, T, 8 * G, 8, u, RAGGED, edit=edit), 2.0 ** -8)
+
+
+@pytest.mark.parametrize("T,G", ROWS)
+def test_batch_of_more_than_32_sequences(rng, T, G):
+    """75 sequences of short, very short and no context; items of one tile beside items of several."""
+    lens = rng.integers(0, 300, 75)
+    lens[[3, 31, 32, 64, 70]] = [0, 128 - T, 129 - T, 0, 900]
+    _check(_case(rng, 75, T, 4 * G, 4, 4, lens, least=2.0))
+
+
+def test_few_long_sequences_cut_into_runs(rng):
+    """Every item cut into many runs, some of which begin in the middle of one item and end in the middle of the next."""
+    _check(_case(rng, 2, 8, 16, 8, 4, [9999, 6001]))
+
+
+# ------------------------------------------------------------------------------------------------ verify_tree
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("V,dtype", [(65536, torch.float32), (65537, torch.float32), (70001, torch.bfloat16), (128256, torch.float32),
+                                     (200003, torch.bfloat16)])
+def test_verify_large_vocabularies(rng, V, dtype, drawn):
+    """More than 512 entries to a warp."""
+    p, d, tokens, parents, u = _verify_case(rng, 3, 6, V, drawn, near=2.0)
+    parents[0, 1:] = 0                                         # a chain of rejections
+    _check_verify(p, d, tokens, parents, u, dtype)
