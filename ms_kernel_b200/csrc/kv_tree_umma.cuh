@@ -12,10 +12,13 @@
 //     operand A; the factor 2^e_max is applied to the scores.  Values become fp16 operands q 2^(e + 1) in shared memory,
 //     [key][channel] with the channel as the contiguous (M) dimension.
 //   * One warp looks at a tile's value exponents first: a tile that holds one outside -25 .. 3 (2^-19 to 2^10 in magnitude) is done
-//     in bf16 instead, values and probabilities: the range of fp32 at eight digits, so that a row is not touched by the range
-//     of a key it does not see.  (Exponents from -100 down, the quantiser's for a block of zeros among them, count as zeros beside the others.)
-//   * Queries are staged once per item, rotated in fp32, scaled by a power of two into fp16 (11 digits; the bf16 query has 8, its
-//     rotation more).  Probabilities are fp16 (11 digits), 2^7 above the reference's scale so that they reach down to 2^-31.
+//     in bf16 instead, values and probabilities: the range of fp32 (values exact, probabilities at sixteen digits), so that a row is
+//     not touched by the range of a key it does not see.  (Exponents from -100 down, the quantiser's for a block of zeros among them, count as zeros beside the others.)
+//   * Queries are staged once per item, rotated in fp32, scaled by a power of two and held as two fp16 numbers, the leading eleven digits and
+//     what they leave: 22 digits.  So are probabilities (two bf16 numbers beside values in bf16), 2^7 above the reference's scale so that
+//     they reach down to 2^-31.  With one number each the result before its rounding was off by 1.2e-4 (beside values in bf16 by 1.1e-3);
+//     now by less than 2e-5, for 12 % more time (16 sequences of 16 nodes, below), 9 % (61 nodes), 2 % (8 nodes over 509 keys).  The
+//     second numbers of the probabilities are further columns of the same products: the values are read once.
 //   * Eight softmax warps, thread = (key, half of the rows), four up to 32 rows.  The maximum is lazy: a row's reference moves only when a score
 //     exceeds it by more than 2^8 -- one vote per tile of the four warps that hold the row -- and then the accumulators of the
 //     rows concerned are rescaled in tensor memory.  Sums and accumulators are fp32.
@@ -42,14 +45,19 @@ constexpr int KTU_DEC_WARPS = 16, KTU_KEYS = 128, KTU_ROWS = 64;
 // Softmax warps: two halves of the rows by four quarters of the keys; up to 32 rows one set of four (a warp's work is mostly its waits then).
 __host__ __device__ constexpr int ktu_soft_warps(int nr) { return nr > 32 ? 8 : 4; }
 __host__ __device__ constexpr int ktu_threads(int nr) { return (KTU_DEC_WARPS + ktu_soft_warps(nr) + 4) * 32; }       // and four single ones
-constexpr int KTU_COL_O = 0, KTU_COL_S = 64, KTU_COL_K = 192, KTU_COLS = 512;       // tensor memory columns: O, two S, two K (320 used)
-constexpr int KTU_V = 0, KTU_P = 2 * 32768, KTU_Q = KTU_P + 2 * 16384;               // shared memory: values, probabilities, queries, ring
+constexpr int KTU_COL_O = 0, KTU_COL_S = 128, KTU_COL_K = 256, KTU_COLS = 512;      // tensor memory columns: two O, two S, two K (384 used)
+// Shared memory: two buffers of values, probabilities, queries, ring.  Probabilities and queries are stored as two numbers each, the
+// leading digits and what they leave.  Probabilities of up to 32 rows: two buffers, the second numbers of a key right behind the
+// first; 64 rows: one buffer, the second numbers in the half that follows (two buffers leave two tiles for the ring: 423 us against 408).
+constexpr int KTU_V = 0, KTU_P = 2 * 32768, KTU_Q = KTU_P + 32768;
+__host__ __device__ constexpr int ktu_p_buffers(int nr) { return nr > 32 ? 1 : 2; }
+__host__ __device__ constexpr int ktu_p_second(int nr) { return nr > 32 ? 16384 : nr * 2; }
 constexpr int KTU_PART = 132;                                                       // floats of a row's partial result: acc, m, l, padding
 __host__ __device__ constexpr int ktu_ub(int u) { return 4 * (8 - u); }              // bytes of a block: upper codes, shared codes (and an exponent)
 __host__ __device__ constexpr int ktu_sb(int u) { return 2 * u; }
-__host__ __device__ constexpr int ktu_stages(int u) { return u == 4 ? 4 : 3; }
+__host__ __device__ constexpr int ktu_stages(int u, int nr) { return u == 4 && nr <= 32 ? 4 : 3; }
 __host__ __device__ constexpr int ktu_stage_bytes(int u) { return 2 * 4 * KTU_KEYS * (ktu_ub(u) + ktu_sb(u) + 1); }
-__host__ __device__ constexpr int ktu_smem_bytes(int u, int nr) { return KTU_Q + nr * 256 + ktu_stages(u) * ktu_stage_bytes(u) + 1024; }
+__host__ __device__ constexpr int ktu_smem_bytes(int u, int nr) { return KTU_Q + nr * 512 + ktu_stages(u, nr) * ktu_stage_bytes(u) + 1024; }
 constexpr int KTU_V_BITS = 1;                                                       // values are held times 2
 constexpr float KTU_P_BITS = 7.0f, KTU_MOVE = 15.0f;                                // 2^7 at the reference, which moves at 2^15
 
@@ -349,6 +357,7 @@ template <int U, int NR>
 __global__ void __launch_bounds__(ktu_threads(NR), 1)
 kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32) {
     chain_wait();
+    constexpr int PB = ktu_p_buffers(NR);
     constexpr int SW = ktu_soft_warps(NR), NC = NR / (SW / 4);    // softmax warps; columns (query rows) of a thread in the softmax
     constexpr int WARP_MMA = KTU_DEC_WARPS + SW, WARP_COPY = WARP_MMA + 1, WARP_SCOUT = WARP_MMA + 2, WARPS = WARP_MMA + 4;
     extern __shared__ uint8_t ktu_smem_raw[];
@@ -433,9 +442,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     }
     const KtuCursor start = cur;
 
-    constexpr int UB = ktu_ub(U), SB = ktu_sb(U), NST = ktu_stages(U);
+    constexpr int UB = ktu_ub(U), SB = ktu_sb(U), NST = ktu_stages(U, NR);
     constexpr int K_SH = 4 * KTU_KEYS * UB, K_SC = K_SH + 4 * KTU_KEYS * SB, V_UP = K_SC + 4 * KTU_KEYS, V_SC = V_UP + K_SC;
-    const uint32_t ring = sbase + KTU_Q + NR * 256;               // stages: upper, shared codes and exponents of the keys, of the values
+    const uint32_t ring = sbase + KTU_Q + NR * 512;               // stages: upper, shared codes and exponents of the keys, of the values
     const uint32_t vrow = (sbase + KTU_V + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;      // with the swizzle of chunk 0
 
     // A bounded wait of the whole warp.  Where one runs out, it sets sh.abort: from then on no wait waits any more and all roles go on
@@ -511,8 +520,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int p = ktu_place<U>(lane * 4 + i);
-                        const __half h = __float2half_rn(bad >> k & 1 ? 0.0f : v[k][i] * up);
-                        *reinterpret_cast<__half*>(smem + KTU_Q + (p >> 6) * (NR * 128) + r * 128 + ((((p >> 3) & 7) ^ (r & 7)) << 4) + (p & 7) * 2) = h;
+                        const float x = bad >> k & 1 ? 0.0f : v[k][i] * up;
+                        const __half h = __float2half_rn(x);
+                        __half* const to = reinterpret_cast<__half*>(smem + KTU_Q + (p >> 6) * (NR * 128) + r * 128 + ((((p >> 3) & 7) ^ (r & 7)) << 4) + (p & 7) * 2);
+                        to[0] = h;
+                        to[NR * 128] = __float2half_rn(x - __half2float(h));
                     }
                     if (lane == 0) sh.qf[seg & 3][r] = bad >> k & 1 ? __int_as_float(0x7FC00000) : exp2_int(e - 10);
                 }
@@ -651,8 +663,8 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     for (int c = 0; c < NC; ++c)
                         if (!(vis >> c & 1)) x[c] = -INFINITY;
             };
-            // the product before the last has read this tile's buffer of the probabilities
-            if (j > 1) wait(sh.pempty[j & 1], (uint32_t)(j - 2) >> 1);
+            // the product that read this tile's buffer of the probabilities is done
+            if (j >= PB) wait(sh.pempty[(j - PB) & 1], (uint32_t)(j - PB) >> 1);
             bool moved = false;
 #pragma unroll 1
             for (;;) {
@@ -698,15 +710,16 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 tc_fence_after();
                 if (n_seg > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < NC; c += 8) {
+                    for (int c = 0; c < 2 * NC; c += 8) {         // both accumulators of a row
+                        const int r = half * NC + c % NC, col = r + (c < NC ? 0 : NR);
                         float o[8];
-                        ktu_ld8(tlane + KTU_COL_O + half * NC + c, o);
+                        ktu_ld8(tlane + KTU_COL_O + col, o);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const float al = sh.alpha[half * NC + c + k];
+                            const float al = sh.alpha[r + k];
                             o[k] = al == 0.0f ? 0.0f : o[k] * al;
                         }
-                        ktu_st8(tlane + KTU_COL_O + half * NC + c, o);
+                        ktu_st8(tlane + KTU_COL_O + col, o);
                     }
 #pragma unroll
                     for (int c = 0; c < NC; c += 2) {
@@ -720,22 +733,31 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             }
             tc_fence_before();
             arrive(sh.sempty[j & 1]);
-            // ---- probabilities to shared memory, in the type of the tile's values ----
-            const uint32_t pr = prow + (j & 1) * 16384;
+            // ---- probabilities to shared memory, in the type of the tile's values: the leading digits, then what they leave ----
+            const uint32_t pr = prow + (PB == 2 ? (j & 1) * 16384 : 0), keep = wide ? 0xFFFF0000u : 0xFFFFE000u;
+            const uint64_t minus = pack2(-1.0f, -1.0f);
 #pragma unroll
             for (int c = 0; c < NC; c += 8) {
-                uint32_t w[4];
+                uint32_t w[4], w2[4];
 #pragma unroll
                 for (int k = 0; k < 8; k += 2) {
                     x[c + k] = ktu_exp2(x[c + k]);
                     x[c + k + 1] = ktu_exp2(x[c + k + 1]);
                     l[(c + k) / 2] = add2(l[(c + k) / 2], pack2(x[c + k], x[c + k + 1]));
-                    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(x[c + k + 1]), "f"(x[c + k]));
+                    const float h0 = __uint_as_float(__float_as_uint(x[c + k]) & keep), h1 = __uint_as_float(__float_as_uint(x[c + k + 1]) & keep);
+                    float r0, r1;
+                    unpack2(fma2(pack2(h0, h1), minus, pack2(x[c + k], x[c + k + 1])), r0, r1);
+                    if (wide) {
+                        w[k >> 1] = prmt(__float_as_uint(h0), __float_as_uint(h1), 0x7632u);
+                        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w2[k >> 1]) : "f"(r1), "f"(r0));
+                    } else {
+                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(h1), "f"(h0));
+                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w2[k >> 1]) : "f"(r1), "f"(r0));
+                    }
                 }
-                if (wide)
-#pragma unroll
-                    for (int k = 0; k < 8; k += 2) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k >> 1]) : "f"(x[c + k + 1]), "f"(x[c + k]));
-                sts128(pr ^ (half * (NC / 8) + c / 8) << 4, w[0], w[1], w[2], w[3]);
+                const uint32_t to = pr ^ (half * (NC / 8) + c / 8) << 4;
+                sts128(to, w[0], w[1], w[2], w[3]);
+                sts128(NR > 32 ? to + ktu_p_second(NR) : to ^ ktu_p_second(NR), w2[0], w2[1], w2[2], w2[3]);
             }
             fence_async_smem();
             tc_fence_before();
@@ -774,10 +796,12 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 constexpr float V_SCALE = 1.0f / (1 << KTU_V_BITS);
 #pragma unroll 1
                 for (int c = half * NC; c < min(half * NC + NC, rows); c += 8) {
-                    float o[8];
+                    float o[8], o2[8];
                     ktu_ld8(tlane + KTU_COL_O + c, o);
+                    ktu_ld8(tlane + KTU_COL_O + NR + c, o2);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
+                        o[k] += o2[k];
                         const int64_t at = sh.row[c + k] + ch;
                         if (!whole) {
                             a.partial[at] = o[k] * V_SCALE;
@@ -799,7 +823,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     if (warp == WARP_MMA) {
         // ================================ MMAs ================================
         const uint32_t idesc_qk = ktu_idesc(NR, 0, 0), hi = ktu_desc_hi(1024);
-        const uint32_t q_lo = umma_desc_lo(sbase + KTU_Q, 16), v_lo = umma_desc_lo(sbase + KTU_V, 16384), p_lo = umma_desc_lo(sbase + KTU_P, 8192);
+        const uint32_t q_lo = umma_desc_lo(sbase + KTU_Q, 16), v_lo = umma_desc_lo(sbase + KTU_V, 16384), p_lo = umma_desc_lo(sbase + KTU_P, 16384);
         int seg = -1;
         KtuCursor ahead = cur;                                    // of the scores' product, one tile in front
         auto issue_qk = [&](int j) {
@@ -812,8 +836,8 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             tc_fence_after();
             if (elect_lane()) {
 #pragma unroll 1
-                for (int s = 0; s < 8; ++s)
-                    ktu_mma_ts(tm + KTU_COL_S + (j & 1) * 64, tm + KTU_COL_K + (j & 1) * 64 + 8 * s,
+                for (int s = 0; s < 16; ++s)                      // keys by the queries' first numbers, by their second ones
+                    ktu_mma_ts(tm + KTU_COL_S + (j & 1) * 64, tm + KTU_COL_K + (j & 1) * 64 + 8 * (s & 7),
                                q_lo + (s >> 2) * (NR * 8) + (s & 3) * 2, hi, idesc_qk, s > 0);
                 if (!(a.skip_stage == j && blockIdx.x == 0)) tc_commit(smem_u32(&sh.sfull[j & 1]));
             }
@@ -828,11 +852,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 wait(sh.vfull[j & 1], (uint32_t)j >> 1);
                 wait(sh.pfull[j & 1], (uint32_t)j >> 1);
                 tc_fence_after();
-                const uint32_t id = ktu_idesc(NR, sh.wide[j & 7] ? 1u : 0u, 1u);
+                const uint32_t id = ktu_idesc(2 * NR, sh.wide[j & 7] ? 1u : 0u, 1u);
                 if (elect_lane()) {
 #pragma unroll 1
-                    for (int s = 0; s < 8; ++s)
-                        ktu_mma_ss(tm + KTU_COL_O, v_lo + (j & 1) * 2048 + s * 128, hi, p_lo + (j & 1) * 1024 + s * 128, hi, id, !first || s > 0);
+                    for (int s = 0; s < 8; ++s)                   // values by the probabilities' first and second numbers, side by side
+                        ktu_mma_ss(tm + KTU_COL_O, v_lo + (j & 1) * 2048 + s * 128, hi, p_lo + (PB == 2 ? (j & 1) * 1024 : 0) + s * 128, hi, id, !first || s > 0);
                     tc_commit(smem_u32(&sh.vempty[j & 1]));
                     tc_commit(smem_u32(&sh.pempty[j & 1]));
                 }

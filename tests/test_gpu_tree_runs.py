@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from conftest import F32_REL_FRO_TOL
 from oracle import tree_oracle as tro
 from test_gpu_tree import _bf, _bound, _cache, _check_verify, _i32, _random_parents, _verify_case
 
@@ -157,6 +158,42 @@ def test_batch_of_more_than_32_sequences(rng, T, G):
 def test_few_long_sequences_cut_into_runs(rng):
     """Every item cut into many runs, some of which begin in the middle of one item and end in the middle of the next."""
     _check(_case(rng, 2, 8, 16, 8, 4, [9999, 6001]))
+
+
+def _fp32(c, q, mask, Lk, lens):
+    """The result before its rounding to bf16 (float32 output of the C ABI)."""
+    from ms_kernel_b200 import _lib
+    L, (B, T, Hq, _) = _lib.lib(), q.shape
+    qd, ld = _bf(q), _i32(lens)
+    out, of = torch.empty(q.shape, dtype=torch.bfloat16, device="cuda"), torch.empty(q.shape, device="cuda")
+    n = L.msaq_kv_tree_workspace(B, T, Hq, c.Hkv, Lk, D)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    _lib.check(L.msaq_kv_tree_attention(qd.data_ptr(), *[t.data_ptr() for t in (*c.k, *c.v)], out.data_ptr(), of.data_ptr(), ld.data_ptr(),
+                                        mask.data_ptr(), T, B, T, Hq, c.Hkv, Lk, D, 4, c.u, c.gs, c.Lcap, 1, ws.data_ptr(), n,
+                                        torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(of.to(torch.bfloat16), out)
+    return of.double().cpu().numpy()
+
+
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("u", [4, 3, 2])
+@pytest.mark.parametrize("T,G", ROWS)
+def test_result_before_its_rounding(rng, T, G, u, far):
+    """As near to 64 bits as the framework's other kernels before their rounding to bf16 (F32_REL_FRO_TOL), values far apart or not.
+    Elementwise: a probability is held to 2^-20 of itself (2^-15 beside far values), a query element to 2^-21, sums to 2^-18, the
+    smallest numbers of fp16 are 2^-31 of the largest probability."""
+    def edit(K, V):
+        V[:, ::2, ::300] *= 2.0 ** 12
+        V[:, 1::2, 70::500] *= 2.0 ** -26
+
+    c, q, mask, lens, seen = _case(rng, 10, T, 8 * G, 8, u, RAGGED, edit=edit if far else None)
+    got = _fp32(c, q, mask, int(max(lens)) + T, lens)
+    ref, mag, big, all_v = _plain(q, c, lens, seen)
+    err, p = np.abs(got - ref), 2.0 ** -15 if far else 2.0 ** -20
+    lim = mag * (2 * p + 2 * 2.0 ** -21 * big[..., None] + 2.0 ** -18 * (1 + big[..., None])) + 2.0 ** -31 * all_v
+    assert np.linalg.norm(err) <= F32_REL_FRO_TOL * np.linalg.norm(ref)
+    assert (err <= lim).all(), "worst %.3f of the bound" % (err / lim).max()
 
 
 # ------------------------------------------------------------------------------------------------ verify_tree
