@@ -79,6 +79,7 @@ kv_tree_generic_kernel(const KvTreeArgs a) {
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) acc[i] = 0.0f;
     const int64_t head_base = ((int64_t)b * a.Hkv + hk) * a.NB;
+    const float lift = (float)(33 - __clz(a.Lk));             // probabilities below 1 / (2 Lk): the sum over all keys stays finite where the average does
 
     for (int c0 = j0; c0 < j1; c0 += KTG_KEYS) {
         __syncthreads();                                      // the tile before is read
@@ -111,8 +112,8 @@ kv_tree_generic_kernel(const KvTreeArgs a) {
         }
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = exp2f(m - base);
+        const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new + lift;
+        const float alpha = m == -INFINITY ? 0.0f : exp2f(m - m_new);
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {

@@ -9,11 +9,14 @@
 //     copies, three or four tiles ahead (with one tile ahead in registers the loads' latency alone held the kernel to 2.4 TB/s).
 //   * Two teams of eight decode warps take alternate tiles, thread = (key, two 32-blocks).  Keys become fp16 operands q 2^(e - e_max) relative to the
 //     largest exponent of THEIR row (exact down to 2^-24, 2^-31 of the row's largest value below) and go to tensor memory as
-//     operand A; the factor 2^e_max is applied to the scores.  Values become fp16 operands q 2^(e + 1) in shared memory,
+//     operand A; the factor 2^e_max is applied to the scores.  Values become fp16 operands q 2^(e - 1) in shared memory,
 //     [key][channel] with the channel as the contiguous (M) dimension.
-//   * One warp looks at a tile's value exponents first: a tile that holds one outside -25 .. 3 (2^-19 to 2^10 in magnitude) is done
+//   * One warp looks at a tile's value exponents first: a tile that holds one outside -23 .. 5 (2^-17 to 2^12 in magnitude) is done
 //     in bf16 instead, values and probabilities: the range of fp32 (values exact, probabilities at sixteen digits), so that a row is
-//     not touched by the range of a key it does not see.  (Exponents from -100 down, the quantiser's for a block of zeros among them, count as zeros beside the others.)
+//     not touched by the range of a key it does not see.  From the first tile on whose values could take the sums beyond fp32 (2^110 / Lk)
+//     the references of the item are 2^16 Lk lower: an average of finite values is finite.  A key with a block of exponent 122 or more
+//     (127 is what infinities are written as) makes the rows that attend it NaN.  Exponents from -106 down, the
+//     quantiser's for everything below 2^-99, zeros among them, count as zeros beside the others.
 //   * Queries are staged once per item, rotated in fp32, scaled by a power of two and held as two fp16 numbers, the leading eleven digits and
 //     what they leave: 22 digits.  So are probabilities (two bf16 numbers beside values in bf16), 2^7 above the reference's scale so that
 //     they reach down to 2^-31.  With one number each the result before its rounding was off by 1.2e-4 (beside values in bf16 by 1.1e-3);
@@ -58,8 +61,14 @@ __host__ __device__ constexpr int ktu_sb(int u) { return 2 * u; }
 __host__ __device__ constexpr int ktu_stages(int u, int nr) { return u == 4 && nr <= 32 ? 4 : 3; }
 __host__ __device__ constexpr int ktu_stage_bytes(int u) { return 2 * 4 * KTU_KEYS * (ktu_ub(u) + ktu_sb(u) + 1); }
 __host__ __device__ constexpr int ktu_smem_bytes(int u, int nr) { return KTU_Q + nr * 512 + ktu_stages(u, nr) * ktu_stage_bytes(u) + 1024; }
-constexpr int KTU_V_BITS = 1;                                                       // values are held times 2
 constexpr float KTU_P_BITS = 7.0f, KTU_MOVE = 15.0f;                                // 2^7 at the reference, which moves at 2^15
+// What a tile's value exponents make of it: values and probabilities in fp16, in bf16, or in bf16 with the item's probabilities that much
+// lower, from here to its end.  With lg = the bits of Lk: a value is below 2^(e + 8), a probability at most 2^15, so that the sum
+// over Lk keys stays below 2^127 up to e = 103 - lg, and for any value with probabilities 2^(16 + lg) lower.
+constexpr int KTU_NARROW = 0, KTU_WIDE = 1, KTU_HUGE = 2;
+__device__ __forceinline__ int ktu_huge_from(int Lk) { return 104 - (32 - __clz(Lk)); }
+__device__ __forceinline__ float ktu_huge_bits(int Lk) { return (float)(16 + 32 - __clz(Lk)); }
+constexpr int KTU_TOP = 121;                                                        // the quantiser's largest exponent of finite values; half of them is finite whatever the codes
 
 // Upper half of a shared-memory matrix descriptor with 128-byte swizzle; the lower half is umma_desc_lo(address, lbo).
 // MN-major: rows of 64 elements (128 bytes), 8 of them (K) to a 1024-byte atom, atoms `sbo` bytes apart in K and `lbo` in M or N.
@@ -341,7 +350,7 @@ struct __align__(16) KtuShared {
     uint32_t tmem;
     int len;                                                      // of the first tile's sequence
     volatile int abort;
-    int wide[8];                                                  // tile's values (and probabilities) are bf16
+    int wide[8];                                                  // KTU_NARROW, KTU_WIDE, KTU_HUGE of the tile
     uint64_t mask[KT_MAX_T];
     float qf[4][KTU_ROWS], qscale[4];                             // score factors 2^x of the query rows; of all rows where they are the same
     int same[4], qtop[KTU_DEC_WARPS], qlow[KTU_DEC_WARPS];
@@ -543,8 +552,13 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             const uint32_t se = st + key;
             const int e0 = lds_s8<0>(se + K_SC + 2 * half * KTU_KEYS), e1 = lds_s8<KTU_KEYS>(se + K_SC + 2 * half * KTU_KEYS);
             const int emax = max(max(e0, e1), max((int)lds_s8<0>(se + K_SC + (2 - 2 * half) * KTU_KEYS), (int)lds_s8<KTU_KEYS>(se + K_SC + (2 - 2 * half) * KTU_KEYS)));
-            if (half == 0) sh.ck[j & 3][key] = a.sm_scale_log2 * exp2_int(emax);
-            const bool wide = sh.wide[j & 7] != 0;
+            const bool wide = sh.wide[j & 7] != KTU_NARROW;
+            if (half == 0) {
+                float f = a.sm_scale_log2 * exp2_int(emax);
+                if (wide && max(max((int)lds_s8<0>(se + V_SC), (int)lds_s8<KTU_KEYS>(se + V_SC)), max((int)lds_s8<2 * KTU_KEYS>(se + V_SC), (int)lds_s8<3 * KTU_KEYS>(se + V_SC))) > KTU_TOP)
+                    f = __int_as_float(0x7FC00000);               // no number: what attends this key is none either
+                sh.ck[j & 3][key] = f;
+            }
             if (j > 1) wait(sh.sfull[team], (uint32_t)(j - 2) >> 1);
             tc_fence_after();
             const uint32_t row = vrow + team * 32768 + half * 16384;
@@ -567,7 +581,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         if (j > 1) wait(sh.vempty[team], (uint32_t)(j - 2) >> 1);
                     }
                     // (in bf16: the codes here, their exponent below; out of range otherwise: zeros, or a key that no row attends)
-                    d = wide ? 0 : min(lds_s8<0>(se + V_SC + (2 * half + i - 2) * KTU_KEYS), 4 - KTU_V_BITS) + KTU_V_BITS;
+                    d = wide ? 0 : min(lds_s8<0>(se + V_SC + (2 * half + i - 2) * KTU_KEYS), 5) - 1;
                 }
                 const uint4 sc = lds128(tab + (4 - max(d, -27)) * 16);
                 uint32_t w[16];
@@ -579,7 +593,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     continue;
                 }
                 if (wide) {
-                    const float f = exp2_int(max(-126, min(116, lds_s8<0>(se + V_SC + (2 * half + i - 2) * KTU_KEYS) + KTU_V_BITS)));
+                    const float f = exp2_int(max(-126, min(KTU_TOP, lds_s8<0>(se + V_SC + (2 * half + i - 2) * KTU_KEYS)) - 1));
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {                            // eight digits: exact
                         const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&w[c]));
@@ -602,7 +616,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         const int stid = tid - KTU_DEC_WARPS * 32, htid = stid & 127;             // thread of the role, of its half
         int seg = -1, n_seg = 0;
         bool same = true;                                         // the item's query rows have one score factor
-        float qscale = 1.0f;
+        float qscale = 1.0f, lower = 0.0f;                        // lower: bits that the segment's probabilities are lower by
         uint64_t l[NC / 2];                                       // sums of pairs of rows over this thread's keys
 #pragma unroll 1
         for (int j = 0; j < n_run; ++j) {
@@ -610,6 +624,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             if (j == 0 || cur.t == 0) {
                 ++seg;
                 n_seg = 0;
+                lower = 0.0f;
                 wait(sh.qfull[seg & 3], (uint32_t)seg >> 2);
                 ktu_bar(2, SW * 32);                       // the last item's masks and references are read
                 if (stid < a.T) sh.mask[stid] = a.mask[cur.b * a.mask_stride + stid];
@@ -629,7 +644,8 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             const bool tail = jb + KTU_KEYS > cur.len;            // the tile has nodes of the tree
             wait(sh.kfull[j & 3], (uint32_t)j >> 2);
             const float ck = same ? sh.ck[j & 3][key] * qscale : sh.ck[j & 3][key];
-            const bool wide = sh.wide[j & 7] != 0;
+            const int range = sh.wide[j & 7];
+            const bool wide = range != KTU_NARROW;
             uint32_t vis = 0xFFFFFFFFu;                           // which of this thread's rows attend its key
             if (tail) {
                 const int k = jb + key - cur.len;                 // below 0: in front of the tree
@@ -675,9 +691,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                     top = fmaxf(top, x[c]);
                     top1 = fmaxf(top1, x[c + 1]);
                 }
-                if (moved || !ktu_vote(3 + half, 128, n_seg == 0 || fmaxf(top, top1) > KTU_MOVE)) break;
+                const float drop = range == KTU_HUGE && lower == 0.0f ? ktu_huge_bits(a.Lk) : 0.0f;
+                if (moved || !ktu_vote(3 + half, 128, n_seg == 0 || drop > 0.0f || fmaxf(top, top1) > KTU_MOVE - lower)) break;
                 moved = true;
-                // ---- references move: rows of this half whose maximum of this tile is beyond theirs ----
+                lower += drop;
+                // ---- references move: rows of this half whose maximum of this tile is beyond theirs; all, where they get lower ----
                 if (n_seg > 0) wait(sh.pempty[(j - 1) & 1], (uint32_t)(j - 1) >> 1);  // the accumulators are at rest
 #pragma unroll 1
                 for (int c = 0; c < NC; c += 8) {
@@ -697,14 +715,17 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 if (htid < NC) {
                     const int r = half * NC + htid;
                     const float mx = fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), m = sh.m[r];
-                    float al = 1.0f;
+                    float al = -drop, to = m;
                     float* const rf = reinterpret_cast<float*>(sh.ref4) + r;
                     if (*rf == *rf && mx > -INFINITY && (m == -INFINITY || mx - m > KTU_MOVE - KTU_P_BITS)) {
-                        al = m == -INFINITY ? 0.0f : ktu_exp2(m - mx);
-                        sh.m[r] = mx;
-                        *rf = KTU_P_BITS - mx;
+                        al = m - mx - drop;                       // (-inf: nothing seen yet)
+                        to = mx;
                     }
-                    sh.alpha[r] = al;
+                    if (*rf == *rf && to > -INFINITY) {
+                        sh.m[r] = to;
+                        *rf = KTU_P_BITS - lower - to;
+                    }
+                    sh.alpha[r] = ktu_exp2(al);
                 }
                 ktu_bar(3 + half, 128);
                 tc_fence_after();
@@ -716,8 +737,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         ktu_ld8(tlane + KTU_COL_O + col, o);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const float al = sh.alpha[r + k];
-                            o[k] = al == 0.0f ? 0.0f : o[k] * al;
+                            o[k] *= sh.alpha[r + k];
                         }
                         ktu_st8(tlane + KTU_COL_O + col, o);
                     }
@@ -726,7 +746,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         const float al0 = sh.alpha[half * NC + c], al1 = sh.alpha[half * NC + c + 1];
                         float l0, l1;
                         unpack2(l[c / 2], l0, l1);
-                        l[c / 2] = pack2(al0 == 0.0f ? 0.0f : l0 * al0, al1 == 0.0f ? 0.0f : l1 * al1);
+                        l[c / 2] = pack2(l0 * al0, l1 * al1);
                     }
                     ktu_st_wait();
                 }
@@ -781,11 +801,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 if (htid < NC) {
                     const int r = half * NC + htid;
                     const float s = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
-                    sh.alpha[r] = s == 0.0f ? 0.0f : 1.0f / s;
+                    sh.alpha[r] = s == 0.0f ? 0.0f : 2.0f / s;            // (values are held halved)
                     const int row = r0 + r;
                     sh.row[r] = whole ? (((int64_t)cur.b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 : part + r * KTU_PART;
                     if (!whole) {
-                        a.partial[part + r * KTU_PART + 128] = sh.m[r];
+                        a.partial[part + r * KTU_PART + 128] = sh.m[r] + lower;
                         a.partial[part + r * KTU_PART + 129] = s;
                     }
                 }
@@ -793,7 +813,6 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 wait(sh.pempty[j & 1], (uint32_t)j >> 1);
                 tc_fence_after();
                 const int ch = ktu_element<U>(key);                           // accumulator lane = operand place of the channel
-                constexpr float V_SCALE = 1.0f / (1 << KTU_V_BITS);
 #pragma unroll 1
                 for (int c = half * NC; c < min(half * NC + NC, rows); c += 8) {
                     float o[8], o2[8];
@@ -804,9 +823,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         o[k] += o2[k];
                         const int64_t at = sh.row[c + k] + ch;
                         if (!whole) {
-                            a.partial[at] = o[k] * V_SCALE;
+                            a.partial[at] = o[k];
                         } else if (c + k < rows) {
-                            const float f = sh.alpha[c + k], v = f == 0.0f ? 0.0f : o[k] * V_SCALE * f;
+                            const float f = sh.alpha[c + k], v = f == 0.0f ? 0.0f : o[k] * f;
                             out[at] = __float2bfloat16_rn(v);
                             if (out_f32) out_f32[at] = v;
                         }
@@ -852,7 +871,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 wait(sh.vfull[j & 1], (uint32_t)j >> 1);
                 wait(sh.pfull[j & 1], (uint32_t)j >> 1);
                 tc_fence_after();
-                const uint32_t id = ktu_idesc(2 * NR, sh.wide[j & 7] ? 1u : 0u, 1u);
+                const uint32_t id = ktu_idesc(2 * NR, sh.wide[j & 7] != KTU_NARROW, 1u);
                 if (elect_lane()) {
 #pragma unroll 1
                     for (int s = 0; s < 8; ++s)                   // values by the probabilities' first and second numbers, side by side
@@ -897,20 +916,23 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
     } else if (warp == WARP_SCOUT) {
         // ================================ value exponents ================================
         uint32_t slot = 0, phase = 0;
+        bool huge = false;                                        // of a tile of this item so far
         for (int j = 0; j < n_run; ++j) {
             wait(sh.rfull[slot], phase);
             const uint4 v = lds128<V_SC>(ring + slot * ktu_stage_bytes(U) + lane * 16);            // block lane / 8, keys 16 (lane % 8) ..
             const int valid = cur.len + a.T - cur.t * KTU_KEYS - (lane & 7) * 16;
-            bool far = false;
+            int top = -128, low = 127;                            // of the exponents that are no zeros
             uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
 #pragma unroll 1
             for (int k = 0; k < 8; ++k, lo >>= 8, hi >>= 8) {
                 const int e0 = (int8_t)lo, e1 = (int8_t)hi;
-                far = far || (k < valid && e0 > -100 && (unsigned)(e0 + 24 + KTU_V_BITS) > 28u) ||
-                      (k + 8 < valid && e1 > -100 && (unsigned)(e1 + 24 + KTU_V_BITS) > 28u);
+                if (k < valid && e0 > -106) { top = max(top, e0); low = min(low, e0); }
+                if (k + 8 < valid && e1 > -106) { top = max(top, e1); low = min(low, e1); }
             }
-            far = __any_sync(0xffffffffu, far);
-            if (lane == 0) sh.wide[j & 7] = far;
+            top = __reduce_max_sync(0xffffffffu, top);
+            low = __reduce_min_sync(0xffffffffu, low);
+            huge = (huge && cur.t > 0) || top >= ktu_huge_from(a.Lk);
+            if (lane == 0) sh.wide[j & 7] = huge ? KTU_HUGE : top > 5 || low < -23 ? KTU_WIDE : KTU_NARROW;
             arrive(sh.ready[slot]);
             cur.next(a, groups, B);
             if (++slot == NST) { slot = 0; phase ^= 1u; }
@@ -1014,7 +1036,7 @@ kv_tree_merge_kernel(const KvTreeArgs a, int B, int groups, int blocks, __nv_bfl
             den = fmaf(l[k], w, den);
         }
     }
-    const float f = den == 0.0f ? 0.0f : 1.0f / den;
+    const float f = den == 0.0f ? 0.0f : 2.0f / den;              // (values were held halved)
     const int64_t o = (((int64_t)b * a.T + row / G) * a.Hq + hk * G + row % G) * 128 + 4 * lane;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {

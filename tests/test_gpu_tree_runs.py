@@ -196,6 +196,105 @@ def test_result_before_its_rounding(rng, T, G, u, far):
     assert (err <= lim).all(), "worst %.3f of the bound" % (err / lim).max()
 
 
+def _nodes_only(rng, u, gs, Lcap, T, ctx, K, V, seen, Hq=4):
+    """One sequence, one kv head, given keys and values [ctx + T, 128] -> (result, reference, mag, big, all_v), fp32 and 64 bits."""
+    c = _cache(1, 1, D, Lcap, u, gs, rotate=False)
+    for X, pl in ((K, c.k), (V, c.v)):
+        torch.ops.msaq.kv_write_into(X[None, None].to(torch.bfloat16).contiguous(), *pl, 1, ctx + T, D, 4, 0, Lcap, u, gs, False)
+    q = np.zeros((1, T, Hq, D), np.float32)
+    q[..., 0] = 1                                              # a key's first channel, over sqrt(128), is its score
+    mask = torch.from_numpy(tro.mask_words(seen)).cuda()
+    got = c.attend_tree(_bf(q), mask, ctx + T, _i32([ctx])).double().cpu().numpy()
+    ref, mag, big, all_v = tro.tree_attention(q, [t.cpu().numpy() for t in c.k], [t.cpu().numpy() for t in c.v], u, gs, [ctx], [seen], False)
+    return got, ref, mag, big, all_v
+
+
+# the tuned kernel; another group size, another capacity: the generic one
+KERNELS = [(4, 2, 0), (3, 2, 0), (2, 2, 0), (4, 8, 0), (4, 2, 1)]
+
+
+@pytest.mark.parametrize("u,gs,odd", KERNELS)
+@pytest.mark.parametrize("bits", [100, 110, 118, 120, 124, 126])
+@pytest.mark.parametrize("ctx", [1, 4096])
+def test_large_values_average_to_finite_numbers(rng, u, gs, odd, bits, ctx):
+    """One key of 2^bits, or 4096 of them, and among the nodes one with a weight of 2^-30 and one of 2^-60 in front of them."""
+    T = 4
+    K, V = torch.zeros((ctx + T, D), device="cuda"), torch.ones((ctx + T, D), device="cuda")
+    V[:ctx] *= 2.0 ** bits * (1 + 0.9 * torch.rand((ctx, D), device="cuda"))
+    V[ctx:] = torch.randn((T, D), device="cuda")
+    V[ctx + 1] *= 2.0 ** bits
+    K[ctx + 1, 0], K[ctx + 2, 0] = -235.0, -470.0              # e^(-235 / sqrt(128)) = 2^-30
+    seen = [{0}, {0, 1}, {0, 2}, {3}]
+    got, ref, mag, big, all_v = _nodes_only(rng, u, gs, (ctx + T + 15) // 16 * 16 + odd, T, ctx, K, V, seen)
+    assert np.isfinite(got).all()
+    err, lim = np.abs(got - ref), _bound(ref, mag, big, all_v, 2.0 ** -15)
+    assert (err <= lim).all(), "worst %.3f of the bound" % (err / lim).max()
+
+
+@pytest.mark.parametrize("u,gs,odd", KERNELS)
+@pytest.mark.parametrize("bits", [110, 120, 126])
+def test_small_values_beside_large_ones(rng, u, gs, odd, bits):
+    """Nodes that attend only small values keep their digits beside nodes that attend large ones: a large value with a weight of 2^-30
+    is a large number, the others are as if it were not there."""
+    T, ctx = 6, 0
+    K, V = torch.zeros((T, D), device="cuda"), torch.randn((T, D), device="cuda")
+    V[1] *= 2.0 ** -60
+    V[3] = 2.0 ** bits * (1 + 0.9 * torch.rand(D, device="cuda"))
+    K[3, 0] = -235.0
+    seen = [{0}, {1}, {0, 2}, {2, 3}, {4}, {1, 5}]
+    got, ref, mag, big, all_v = _nodes_only(rng, u, gs, 16 + odd, T, ctx, K, V, seen)
+    err, lim = np.abs(got - ref), _bound(ref, mag, big, all_v, 2.0 ** -15)
+    assert (err <= lim).all(), "worst %.3f of the bound" % (err / lim).max()
+
+
+@pytest.mark.parametrize("T,G", ROWS)
+def test_large_values_in_a_run(rng, T, G):
+    """Large values come up in the middle of some items, in front of and behind tiles of ordinary ones, while references move."""
+    def edit(K, V):
+        V[::2, ::3, 1500:1503] *= 2.0 ** 117
+        V[1::2, 1::3, 64] *= 2.0 ** 121
+        V[0, 2, 5000] *= 2.0 ** 95
+        V[:, :, 200:210] *= 2.0 ** 13
+
+    _check(_case(rng, 10, T, 8 * G, 8, 4, RAGGED, edit=edit, aim=2.0, scale=0.5), 2.0 ** -15)
+
+
+@pytest.mark.parametrize("u", [4, 3, 2])
+def test_values_without_a_finite_number(rng, u):
+    """An infinity: NaN in the rows that attend it, the others as without it.  The largest finite values are numbers."""
+    T, ctx = 5, 3
+    for value in (2.0 ** 127, np.inf, -np.inf):
+        K, V = torch.zeros((ctx + T, D), device="cuda"), torch.randn((ctx + T, D), device="cuda")
+        V[ctx + 2, 77] = value
+        seen = [{0}, {1}, {0, 2}, {2}, {0, 4}]
+        c = _cache(1, 1, D, 16, u, 2, rotate=False)
+        for X, pl in ((K, c.k), (V, c.v)):
+            torch.ops.msaq.kv_write_into(X[None, None].to(torch.bfloat16).contiguous(), *pl, 1, ctx + T, D, 4, 0, 16, u, 2, False)
+        q = _bf(rng.standard_normal((1, T, 4, D)))
+        mask = torch.from_numpy(tro.mask_words(seen)).cuda()
+        got = c.attend_tree(q, mask, ctx + T, _i32([ctx])).float().cpu().numpy()
+        assert np.isfinite(got[0, [0, 1, 4]]).all()
+        if np.isinf(value):
+            assert np.isnan(got[0, 2:4]).all()
+        else:
+            assert np.isfinite(got).all()
+        planes = [[t.cpu().numpy() for t in pl] for pl in (c.k, c.v)]
+        planes[1][0][0, 0, :, ctx + 2] = 0                     # not attended by the others: any finite value will do
+        ref, mag, big, all_v = tro.tree_attention(q.float().cpu().numpy(), *planes, u, 2, [ctx], [seen], False)
+        ok = (np.abs(got - ref) <= _bound(ref, mag, big, all_v, 2.0 ** -15))[0, [0, 1, 4]]
+        assert ok.all()
+
+
+@pytest.mark.parametrize("bits", [-98, -95, -90])
+def test_values_next_to_the_smallest_that_the_format_holds(rng, bits):
+    """The quantiser's smallest block (2^-100 and below) counts as zeros; what is larger counts."""
+    T, ctx = 2, 130
+    K, V = torch.zeros((ctx + T, D), device="cuda"), 2.0 ** bits * (1 + 0.9 * torch.rand((ctx + T, D), device="cuda"))
+    got, ref, mag, big, all_v = _nodes_only(rng, 4, 2, 144, T, ctx, K, V, [{0}, {0, 1}])
+    lim = _bound(ref, mag, big, all_v, 2.0 ** -15) - 1e-30
+    assert (np.abs(got - ref) <= lim).all()
+
+
 # ------------------------------------------------------------------------------------------------ verify_tree
 @pytest.mark.parametrize("drawn", [False, True])
 @pytest.mark.parametrize("V,dtype", [(65536, torch.float32), (65537, torch.float32), (70001, torch.bfloat16), (128256, torch.float32),
