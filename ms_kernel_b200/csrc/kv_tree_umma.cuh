@@ -11,7 +11,7 @@
 //     largest exponent of THEIR row (exact down to 2^-24, 2^-31 of the row's largest value below) and go to tensor memory as
 //     operand A; the factor 2^e_max is applied to the scores.  Values become fp16 operands q 2^(e - 1) in shared memory,
 //     [key][channel] with the channel as the contiguous (M) dimension.
-//   * One warp looks at a tile's value exponents first: a tile that holds one outside -23 .. 5 (2^-17 to 2^12 in magnitude) is done
+//   * One warp looks at the value exponents of a tile's attended keys first: a tile that holds one outside -23 .. 5 (2^-17 to 2^12 in magnitude) is done
 //     in bf16 instead, values and probabilities: the range of fp32 (values exact, probabilities at sixteen digits), so that a row is
 //     not touched by the range of a key it does not see.  From the first tile on whose values could take the sums beyond fp32 (2^110 / Lk)
 //     the references of the item are 2^16 Lk lower: an average of finite values is finite.  A key with a block of exponent 122 or more
@@ -917,17 +917,28 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         // ================================ value exponents ================================
         uint32_t slot = 0, phase = 0;
         bool huge = false;                                        // of a tile of this item so far
+        uint64_t named = 0;                                       // nodes that some node of the sequence attends
+        int whose = -1;                                           // that sequence
         for (int j = 0; j < n_run; ++j) {
+            const int node = cur.t * KTU_KEYS + (lane & 7) * 16 - cur.len;         // of this lane's first key; below 0: in front of the tree
+            if (whose != cur.b && (cur.t + 1) * KTU_KEYS > cur.len) {
+                whose = cur.b;
+                const uint64_t* const words = a.mask + cur.b * a.mask_stride;
+                named = (lane < a.T ? words[lane] : 0ull) | (lane + 32 < a.T ? words[lane + 32] : 0ull);
+                named = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(named >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)named);
+                named &= ~0ull >> (64 - a.T);
+            }
+            // which of the lane's sixteen keys somebody attends
+            const uint32_t keys = node <= -16 ? 0xFFFFu : node < 0 ? (uint32_t)(named << -node) | ((1u << -node) - 1u) : node < 64 ? (uint32_t)(named >> node) : 0u;
             wait(sh.rfull[slot], phase);
             const uint4 v = lds128<V_SC>(ring + slot * ktu_stage_bytes(U) + lane * 16);            // block lane / 8, keys 16 (lane % 8) ..
-            const int valid = cur.len + a.T - cur.t * KTU_KEYS - (lane & 7) * 16;
             int top = -128, low = 127;                            // of the exponents that are no zeros
             uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
 #pragma unroll 1
             for (int k = 0; k < 8; ++k, lo >>= 8, hi >>= 8) {
                 const int e0 = (int8_t)lo, e1 = (int8_t)hi;
-                if (k < valid && e0 > -106) { top = max(top, e0); low = min(low, e0); }
-                if (k + 8 < valid && e1 > -106) { top = max(top, e1); low = min(low, e1); }
+                if (keys >> k & 1 && e0 > -106) { top = max(top, e0); low = min(low, e0); }
+                if (keys >> (k + 8) & 1 && e1 > -106) { top = max(top, e1); low = min(low, e1); }
             }
             top = __reduce_max_sync(0xffffffffu, top);
             low = __reduce_min_sync(0xffffffffu, low);

@@ -295,6 +295,30 @@ def test_values_next_to_the_smallest_that_the_format_holds(rng, bits):
     assert (np.abs(got - ref) <= lim).all()
 
 
+@pytest.mark.parametrize("u,gs,odd", KERNELS)
+@pytest.mark.parametrize("T,ctx", [(6, 45), (6, 126), (64, 100), (33, 0)])
+def test_slots_that_nobody_attends_do_not_matter(rng, T, ctx, u, gs, odd):
+    """Whatever bytes the slots hold that no mask bit names, inside the tree and behind it: the same bits come out."""
+    B, Hq, Hkv, Lcap = 2, 8, 2, (ctx + T + 20) // 16 * 16 + odd
+    c = _cache(B, Hkv, D, Lcap, u, gs)
+    c.fill(*(_bf(rng.standard_normal((B, Hkv, ctx + T, D))) for _ in range(2)))
+    parents = [[-1] + [0 if i % 3 else -1 for i in range(1, T)], [-1] * T]
+    seen = [tro.tree_mask(p) for p in parents]
+    seen[1][T - 1] = {0, T - 1}
+    mask = torch.from_numpy(np.stack([tro.mask_words(s) for s in seen])).cuda()
+    q, lens, outs = _bf(rng.standard_normal((B, T, Hq, D))), _i32([ctx, ctx - ctx // 3]), []
+    for pattern in (None, 0x00, 0x7F, 0x80, 0x5A, 0xFF):
+        if pattern is not None:
+            for b in range(B):
+                n = int(lens[b])
+                free = sorted(set(range(T)) - set().union(*seen[b]))
+                at = torch.tensor([n + j for j in free] + list(range(n + T, Lcap)), device="cuda")
+                for t in (*c.k, *c.v):
+                    t[b, :, :, at] = pattern - 256 if t.dtype == torch.int8 and pattern > 127 else pattern
+        outs.append(c.attend_tree(q, mask, ctx + T, lens))
+        assert torch.isfinite(outs[-1]).all() and torch.equal(outs[0], outs[-1]), pattern
+
+
 # ------------------------------------------------------------------------------------------------ verify_tree
 @pytest.mark.parametrize("drawn", [False, True])
 @pytest.mark.parametrize("V,dtype", [(65536, torch.float32), (65537, torch.float32), (70001, torch.bfloat16), (128256, torch.float32),
