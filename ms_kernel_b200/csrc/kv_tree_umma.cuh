@@ -900,6 +900,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         int issued = 0;
         for (int j = 0; j < n_run; ++j) {
             wait(sh.rempty[slot], phase);
+            // After a give-up the slot may still be on its way or being read: no more copies, and only what was issued is waited for below.  (The
+            // other roles wait for nothing then, and this warp meets them at the block's last barrier only.)
+            if (__any_sync(0xffffffffu, sh.abort)) break;
             const int n = min(KTU_KEYS, (cur.len + a.T - cur.t * KTU_KEYS + 15) & ~15);            // whole groups of 16 (so is the capacity)
             const int64_t row = (((int64_t)cur.b * a.Hkv + cur.hk) * 4 + i) * a.Lcap + cur.t * KTU_KEYS;
             const uint32_t bar = smem_u32(&sh.rfull[slot]);

@@ -319,6 +319,37 @@ def test_slots_that_nobody_attends_do_not_matter(rng, T, ctx, u, gs, odd):
         assert torch.isfinite(outs[-1]).all() and torch.equal(outs[0], outs[-1]), pattern
 
 
+@pytest.mark.parametrize("stage", [0, 1, 4, 7])
+@pytest.mark.parametrize("T,G,u", [(8, 2, 4), (16, 2, 3), (16, 4, 4), (47, 3, 2)])
+def test_give_up_in_the_middle_of_a_run(rng, T, G, u, stage):
+    """The first thread block's product of tile `stage` is never signalled: the items that its run touches are NaN, all others are as
+    ever, the status word says so, and the next call is right."""
+    import cabi
+    c, q, mask, lens, _ = _case(rng, 10, T, 8 * G, 8, u, RAGGED, least=8.0)
+    qd, ld, Lk = _bf(q), _i32(lens), int(max(lens)) + T
+    want = c.attend_tree(qd, mask, Lk, ld)
+    run = _tiles(lens, T, 8, G) // torch.cuda.get_device_properties(0).multi_processor_count
+    assert run > stage
+    torch.ops.msaq.wait_status(True)
+    with cabi.options({3: 4096, 4: stage}):
+        got = c.attend_tree(qd, mask, Lk, ld)
+        torch.cuda.synchronize()
+    assert torch.ops.msaq.wait_status(True) == 4
+    R, tile = T * G, 0
+    rows = 16 if R <= 16 else 32 if R <= 32 else 64
+    for b in range(len(lens)):
+        for hk in range(8):
+            x, y = (t[b, :, hk * G:(hk + 1) * G].reshape(R, D) for t in (got, want))
+            for r0 in range(0, R, rows):
+                if tile < run:
+                    assert torch.isnan(x[r0:r0 + rows]).all(), (b, hk, r0)
+                else:
+                    assert torch.equal(x[r0:r0 + rows], y[r0:r0 + rows]), (b, hk, r0)
+                tile += -(-(int(lens[b]) + T) // 128)
+    assert torch.equal(c.attend_tree(qd, mask, Lk, ld), want)
+    assert torch.ops.msaq.wait_status(True) == 0
+
+
 # ------------------------------------------------------------------------------------------------ verify_tree
 @pytest.mark.parametrize("drawn", [False, True])
 @pytest.mark.parametrize("V,dtype", [(65536, torch.float32), (65537, torch.float32), (70001, torch.bfloat16), (128256, torch.float32),
