@@ -132,6 +132,7 @@ extern "C" int msaq_kv_tree_attention(const void* q, const int8_t* ks, const uin
     if (reinterpret_cast<uintptr_t>(mask) & 7) return fail(MSAQ_ERR_ARG, "mask must be 8-byte aligned");
     if ((reinterpret_cast<uintptr_t>(ku) | reinterpret_cast<uintptr_t>(vu)) & 3)
         return fail(MSAQ_ERR_ARG, "upper planes must be 4-byte aligned");
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(MSAQ_ERR_ARG, "workspace must be 16-byte aligned");
     if (int rc = require_sm100()) return rc;
     const size_t need = msaq_kv_tree_workspace(B, T, H, Hkv, Lk, D);
     if (!workspace || workspace_bytes < need)

@@ -161,3 +161,17 @@ def test_oracle_verification_keeps_the_targets_distribution(drawn):
         path, token = tro.verify_tree(target, tokens, [-1, 0, 0, 0], rng.random(4), draft if drawn else None)
         got[tokens[path[1]] if len(path) > 1 else token] += 1
     assert np.abs(got / n - p).max() < 0.0125
+
+
+def test_tree_attention_refuses_a_workspace_that_is_not_aligned():
+    """Partial results are read sixteen bytes at a time."""
+    from ms_kernel_b200 import _lib
+    L, one = _lib.lib(), 16
+
+    def call(ws):
+        return L.msaq_kv_tree_attention(one, *[one] * 3, *[one] * 3, one, None, None, one, 0, 1, 8, 8, 2, 64, 128, 4, 4, 2, 64, 1, ws, 1 << 40, None)
+
+    for ws in (one + 1, one + 4, one + 8):
+        assert call(ws) == -1
+    if not torch.cuda.is_available():
+        assert call(one) == -5 and call(None) == -5
