@@ -260,6 +260,8 @@ class KVCache:
         B, T = int(qkv.shape[0]), int(qkv.shape[1])
         if B != self.B:
             raise ValueError("qkv has %d sequences, the cache %d" % (B, self.B))
+        if pos is not None and pos.dim() == 2 and tuple(pos.shape) != (B, T):
+            raise ValueError("pos must be [B, T] = [%d, %d], not %s" % (B, T, list(pos.shape)))
         start_t, start_i = (None, int(start)) if isinstance(start, int) else (start, 0)
         cos, sin = (None, None) if rope is None else (rope[0], rope[1])
         return _OPS.kv_write_qkv(qkv, *self.k, *self.v, start_t, pos, counts, q_gain, k_gain, cos, sin, B, T, int(Hq), self.Hkv,

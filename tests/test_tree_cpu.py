@@ -175,3 +175,15 @@ def test_tree_attention_refuses_a_workspace_that_is_not_aligned():
         assert call(ws) == -1
     if not torch.cuda.is_available():
         assert call(one) == -5 and call(None) == -5
+
+
+def test_write_qkv_refuses_positions_of_another_shape():
+    """[T, B] has as many elements as [B, T]: taken as it stands, it would give most tokens another token's position."""
+    from ms_kernel_b200 import ops
+    cache = ops.KVCache(2, 2, 128, 32, 4, 2, "cpu")
+    qkv = torch.zeros(2, 3, 8 * 128, dtype=torch.bfloat16)
+    for shape in ((3, 2), (1, 6), (2, 4)):
+        with pytest.raises(ValueError):
+            cache.write_qkv(qkv, 4, 0, pos=torch.zeros(shape, dtype=torch.int32))
+    with pytest.raises(RuntimeError):                          # this one is only on the wrong device
+        cache.write_qkv(qkv, 4, 0, pos=torch.zeros(2, 3, dtype=torch.int32))
