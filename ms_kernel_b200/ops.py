@@ -296,9 +296,9 @@ def tree_mask(parents, device="cuda"):
     ancestors; none for a node that is not there), depth counts from the root."""
     import numpy as np
     par = np.asarray(parents, dtype=np.int64)
-    T = par.shape[-1]
-    if par.ndim not in (1, 2) or not 1 <= T <= 64:
+    if par.ndim not in (1, 2) or not 1 <= par.shape[-1] <= 64:
         raise ValueError("parents must be [T] or [B, T] with 1 to 64 nodes")
+    T = par.shape[-1]
     rows = par.reshape(-1, T)
     if (rows[:, 0] != -1).any() or (rows >= np.arange(T)).any() or (rows < -1).any():
         raise ValueError("node 0 is the root (-1), every other node's parent is in front of it or -1")

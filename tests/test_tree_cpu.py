@@ -187,3 +187,9 @@ def test_write_qkv_refuses_positions_of_another_shape():
             cache.write_qkv(qkv, 4, 0, pos=torch.zeros(shape, dtype=torch.int32))
     with pytest.raises(RuntimeError):                          # this one is only on the wrong device
         cache.write_qkv(qkv, 4, 0, pos=torch.zeros(2, 3, dtype=torch.int32))
+
+
+def test_tree_mask_refuses_a_number():
+    from ms_kernel_b200 import ops
+    with pytest.raises(ValueError):
+        ops.tree_mask(-1, "cpu")
