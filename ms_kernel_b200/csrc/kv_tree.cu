@@ -12,21 +12,27 @@ struct TreePlan {
     int S, key_tile, groups, rows;
 };
 
-// Rows per thread block by the rows there are (4 sequences of 32752 keys, in blocks of 16 / 32 / 64: 16 rows 81 / 88 / 105 us, 32 rows
-// 89 against 106; one of 509 keys, 16 rows: 13.1 / 14.7 / 17.2 us); as many runs of the line of tiles as there are SMs, or as there can
-// be tiles.
+// Rows per thread block by the rows there are: blocks of 16 / 32 / 64 took, us, over 4 sequences of 32752 keys and 8 kv heads: 16 rows 93 /
+// 114 / 119, 32 rows 172 / 115 / 120, 64 rows 331 / 214 / 124; 16 sequences of 2000: 38 / 48 / 59, 63 / 52 / 63, 110 / 89 / 66; one of
+// 16000: 16 rows 28 / 34 / 40, 32 rows 38 / 35 / 42.  Fewer where every block still has one tile at most: the keys are decoded more often, by
+// SMs that had nothing to do (one sequence, 8 kv heads: 32 rows over 509 keys 16.1 -> 13.4, 64 rows over 100 keys 19.6 -> 12.1, over
+// 509 20.6 -> 16.3; up to two tiles: 488 rows over 100 keys 23.6 -> 26.9, no) -- not under the hook that stops the first block's
+// products, which then stops all rows of a small item.  As many runs of the line of tiles as there are SMs, or
+// as there can be tiles.
 TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
     TreePlan p;
     const int64_t R = T * (H / Hkv);
     p.rows = R <= 16 ? 16 : R <= 32 ? 32 : 64;
+    const int64_t tiles = B * Hkv * ((Lk + KTU_KEYS - 1) / KTU_KEYS);
+    while (p.rows > 16 && option_test_skip_stage() < 0 && tiles * ((2 * R + p.rows - 1) / p.rows) <= sm_count()) p.rows /= 2;
     p.groups = (int)((R + p.rows - 1) / p.rows);
-    p.S = (int)std::min<int64_t>(sm_count(), B * Hkv * p.groups * ((Lk + KTU_KEYS - 1) / KTU_KEYS));
+    p.S = (int)std::min<int64_t>(sm_count(), tiles * p.groups);
     p.key_tile = KTU_KEYS;
     return p;
 }
 
 // The tuned kernel: head_dim 128, gs = 2, capacity a multiple of 16 (and planes on 16-byte boundaries: bulk copies), tiles counted in 31 bits.
-// (The generic kernel takes 125 instead of 16.7 us at 8 nodes over 509 keys, 16.3 ms instead of 0.35 for 16 sequences of 16 nodes over up to
+// (The generic kernel takes 121 instead of 13.3 us at 8 nodes over 509 keys, 16.2 ms instead of 0.41 for 16 sequences of 16 nodes over up to
 // 32752 keys.)
 bool umma_eligible(int64_t D, int gs, int64_t Lcap, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
     return D == 128 && gs == 2 && Lcap % 16 == 0 && B * Hkv * plan_tree_umma(B, T, H, Hkv, Lk).groups <= INT32_MAX / ((Lk + KTU_KEYS - 1) / KTU_KEYS);

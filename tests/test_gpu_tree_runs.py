@@ -319,6 +319,20 @@ def test_slots_that_nobody_attends_do_not_matter(rng, T, ctx, u, gs, odd):
         assert torch.isfinite(outs[-1]).all() and torch.equal(outs[0], outs[-1]), pattern
 
 
+@pytest.mark.parametrize("T,G", ROWS)
+def test_rows_without_numbers_stay_alone_in_a_run(rng, T, G):
+    """Queries with a NaN or an infinity: NaN in their rows, to the bit the same in all others."""
+    c, q, mask, lens, _ = _case(rng, 10, T, 8 * G, 8, 4, RAGGED)
+    Lk, ld = int(max(lens)) + T, _i32(lens)
+    want = c.attend_tree(_bf(q), mask, Lk, ld)
+    bad = torch.zeros(q.shape[:3], dtype=torch.bool)
+    for b, i, h, d, x in ((0, 0, 0, 5, np.nan), (0, T - 1, 3, 0, np.inf), (4, 3, 8 * G - 1, 127, -np.inf), (6, 5, 1, 64, np.nan), (9, 2, 9, 1, np.inf)):
+        q[b, i, h, d] = x
+        bad[b, i, h] = True
+    got = c.attend_tree(_bf(q), mask, Lk, ld)
+    assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], want[~bad])
+
+
 @pytest.mark.parametrize("stage", [0, 1, 4, 7])
 @pytest.mark.parametrize("T,G,u", [(8, 2, 4), (16, 2, 3), (16, 4, 4), (47, 3, 2)])
 def test_give_up_in_the_middle_of_a_run(rng, T, G, u, stage):
