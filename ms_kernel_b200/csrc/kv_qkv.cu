@@ -4,8 +4,9 @@
 // the verification of a drafted tree: the accepted nodes' rows become neighbours.
 //
 // A head row x with gain g becomes  y = bf16( rope( (x r) g ) ),  r = fl32( (mean(x^2) + eps)^(-1/2) ).  Mean and root are taken
-// in 64 bits: r is then the same number however the sum is split over lanes, and so are the codes that the quantiser derives from
-// y (in 32 bits one key row in about ten thousand would land on other codes).  The remaining steps are fp32 operations,
+// in 64 bits: r then depends on how the sum is split over lanes only where the 64-bit number lies within about 2^-52 of a border
+// between two fp32 numbers, once in 2^28 rows, and so do the codes that the quantiser derives from y (in 32 bits one key row in about ten
+// thousand would land on other codes).  The remaining steps are fp32 operations,
 // each rounded by itself.
 //
 // A token moves 2 D (2 Hq + 2 Hkv) + 2 Hkv NB (UB + SB + 1) bytes and 4 D of tables: 185 MB for 8191 tokens of 32 + 2 x 8 heads (28 us).
@@ -40,8 +41,8 @@ struct QkvArgs {
     int kv_chunks, chunks;               // runs of the key heads (as many of the value heads), of all heads of a token
 };
 
-// (mean + eps)^(-1/2) rounded to fp32: one Newton step of third order in 64 bits on the 32-bit estimate (relative error
-// below 2^-60); a sum beyond the range of fp32 takes the slow root.
+// (mean + eps)^(-1/2) rounded to fp32: one Newton step of third order in 64 bits on the 32-bit estimate (what the series leaves out
+// is below 2^-60, its roundings come to about 2^-52); a sum beyond the range of fp32 takes the slow root.
 __device__ __forceinline__ float norm_factor(double ss, int D, double eps) {
     const double m = ss / (double)D + eps;
     if (!(m > 1e-36 && m < 1e36)) return (float)(1.0 / sqrt(m));

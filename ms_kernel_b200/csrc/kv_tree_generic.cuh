@@ -143,8 +143,7 @@ kv_tree_generic_kernel(const KvTreeArgs a) {
     }
 }
 
-// Merge of the key pieces of a row: weights 2^(m_s - max m).  A NaN in m marks a piece whose wait gave up, or scores that were not
-// numbers: the row is NaN.
+// Merge of the key pieces of a row: weights 2^(m_s - max m).  Scores that were not numbers come through l and acc.
 __global__ void __launch_bounds__(128)
 kv_tree_combine_kernel(const float* __restrict__ partial, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32, int T, int Hq,
                        int Hkv, int D, int S) {
@@ -154,12 +153,7 @@ kv_tree_combine_kernel(const float* __restrict__ partial, __nv_bfloat16* __restr
     const int r = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
     const float* base = partial + (((int64_t)b * Hkv + hk) * R + r) * S * (int64_t)(D + 2);
     float mg = -INFINITY;
-    bool bad = false;
-    for (int s = 0; s < S; ++s) {
-        const float m = base[(int64_t)s * (D + 2) + D];
-        bad = bad || m != m;
-        mg = fmaxf(mg, m);
-    }
+    for (int s = 0; s < S; ++s) mg = fmaxf(mg, base[(int64_t)s * (D + 2) + D]);
     for (int d = threadIdx.x; d < D; d += blockDim.x) {
         float num = 0.0f, den = 0.0f;
         for (int s = 0; s < S; ++s) {
@@ -169,8 +163,7 @@ kv_tree_combine_kernel(const float* __restrict__ partial, __nv_bfloat16* __restr
             num = fmaf(p[d], w, num);
             den = fmaf(p[D + 1], w, den);
         }
-        float v = den == 0.0f ? 0.0f : num / den;
-        if (bad) v = __int_as_float(0x7FC00000);
+        const float v = den == 0.0f ? 0.0f : num / den;
         const int64_t o = (((int64_t)b * T + r / G) * Hq + hk * G + r % G) * D + d;
         out[o] = __float2bfloat16_rn(v);
         if (out_f32) out_f32[o] = v;

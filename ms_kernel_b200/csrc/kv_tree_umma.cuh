@@ -1,4 +1,5 @@
-// Tuned attention for a tree of drafted tokens over a packed cache: gs = 2, head_dim 128, any u, any Hq / Hkv, any capacity.
+// Tuned attention for a tree of drafted tokens over a packed cache: gs = 2, head_dim 128, any u, any Hq / Hkv, capacities
+// that are multiples of 16 (the planes' rows begin on 16-byte boundaries then, as bulk copies need).
 //
 // A thread block (one per SM) takes up to 64 query rows (nodes x the heads of one kv head) against 128 keys at a time, with the KEYS on
 // the tensor cores' wide side:
@@ -36,8 +37,6 @@
 #pragma once
 
 #include <cuda_fp16.h>
-
-#include <type_traits>
 
 #include "tcgen05.cuh"
 #include "kv_tree_generic.cuh"
@@ -114,9 +113,8 @@ __device__ __forceinline__ void ktu_st8(uint32_t taddr, const float* v) {
                  "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
                  : "memory");
 }
-// N accumulator columns (8, 16 or 32) in one access.
+// N accumulator columns (16 or 32) in one access.
 template <int N> __device__ __forceinline__ void ktu_ld(uint32_t taddr, float (&v)[N]);
-template <> __device__ __forceinline__ void ktu_ld<8>(uint32_t taddr, float (&v)[8]) { ktu_ld8(taddr, v); }
 template <> __device__ __forceinline__ void ktu_ld<16>(uint32_t taddr, float (&v)[16]) { tmem_ld16(taddr, v); }
 template <> __device__ __forceinline__ void ktu_ld<32>(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
@@ -867,22 +865,22 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         issue_qk(0);
 #pragma unroll 1
         for (int j = 0; j < n_run; ++j) {
-                if (j + 1 < n_run) issue_qk(j + 1);
-                wait(sh.vfull[j & 1], (uint32_t)j >> 1);
-                wait(sh.pfull[j & 1], (uint32_t)j >> 1);
-                tc_fence_after();
-                const uint32_t id = ktu_idesc(2 * NR, sh.wide[j & 7] != KTU_NARROW, 1u);
-                if (elect_lane()) {
+            if (j + 1 < n_run) issue_qk(j + 1);
+            wait(sh.vfull[j & 1], (uint32_t)j >> 1);
+            wait(sh.pfull[j & 1], (uint32_t)j >> 1);
+            tc_fence_after();
+            const uint32_t id = ktu_idesc(2 * NR, sh.wide[j & 7] != KTU_NARROW, 1u);
+            if (elect_lane()) {
 #pragma unroll 1
-                    for (int s = 0; s < 8; ++s)                   // values by the probabilities' first and second numbers, side by side
-                        ktu_mma_ss(tm + KTU_COL_O, v_lo + (j & 1) * 2048 + s * 128, hi, p_lo + (PB == 2 ? (j & 1) * 1024 : 0) + s * 128, hi, id, !first || s > 0);
-                    tc_commit(smem_u32(&sh.vempty[j & 1]));
-                    tc_commit(smem_u32(&sh.pempty[j & 1]));
-                }
-                __syncwarp();
-                first = cur.t == cur.tiles - 1;
-                cur.next(a, groups, B);
+                for (int s = 0; s < 8; ++s)                   // values by the probabilities' first and second numbers, side by side
+                    ktu_mma_ss(tm + KTU_COL_O, v_lo + (j & 1) * 2048 + s * 128, hi, p_lo + (PB == 2 ? (j & 1) * 1024 : 0) + s * 128, hi, id, !first || s > 0);
+                tc_commit(smem_u32(&sh.vempty[j & 1]));
+                tc_commit(smem_u32(&sh.pempty[j & 1]));
             }
+            __syncwarp();
+            first = cur.t == cur.tiles - 1;
+            cur.next(a, groups, B);
+        }
         // nothing may still write tensor memory when it is returned
         if (elect_lane()) {
             tc_commit(smem_u32(&sh.done));
