@@ -21,8 +21,9 @@
 //   * Queries are staged once per item, rotated in fp32, scaled by a power of two and held as two fp16 numbers, the leading eleven digits and
 //     what they leave: 22 digits.  So are probabilities (two bf16 numbers beside values in bf16), 2^7 above the reference's scale so that
 //     they reach down to 2^-31.  With one number each the result before its rounding was off by 1.2e-4 (beside values in bf16 by 1.1e-3);
-//     now by less than 2e-5, for 12 % more time (16 sequences of 16 nodes, below), 9 % (61 nodes), 2 % (8 nodes over 509 keys).  The
-//     second numbers of the probabilities are further columns of the same products: the values are read once.
+//     now by less than 2e-5 (over 32752 keys by 2.5e-5, 1.5e-6 of the average |v|), for 12 % more time (16 sequences of 16 nodes,
+//     below), 9 % (61 nodes), 2 % (8 nodes over 509 keys).  The second numbers of the probabilities are further columns of the same
+//     products: the values are read once.
 //   * Eight softmax warps, thread = (key, half of the rows), four up to 32 rows.  The maximum is lazy: a row's reference moves only when a score
 //     exceeds it by more than 2^8 -- one vote per tile of the four warps that hold the row -- and then the accumulators of the
 //     rows concerned are rescaled in tensor memory.  Sums and accumulators are fp32.
@@ -30,10 +31,10 @@
 //   * The tiles of all (sequence, kv head, row group) items form one line, cut into equal runs, one per thread block: ragged
 //     batches balance.  An item inside one run is finished there; one that is cut leaves partial results (acc, m, l), merged by a second
 //     kernel in the order of the runs.
-// What bounds it: the instructions of decoding and softmax, 7600 of a warp per tile of 128 keys and 64 rows (two thirds of the issue
-// slots), and the hand-overs between roles; the tensor cores are busy one cycle in seven, HBM one in five.  16 sequences of 16 nodes,
-// 32 / 8 heads, over up to 32752 keys (u = 4): 348 us, 640 MB at 1.8 TB/s; one of 61 nodes, 64 / 8 heads, over 16381 keys: 129 us, 257
-// TFLOP/s; one of 8 nodes over 509 keys: 16.7 us, latency.
+// What bounds it: the instructions of decoding and softmax, 7900 of a warp per tile of 128 keys and 64 rows (61 % of the issue
+// slots), and the hand-overs between roles; the tensor cores are busy one cycle in four, HBM one in five.  16 sequences of 16 nodes,
+// 32 / 8 heads, over up to 32752 keys (u = 4): 373 us, 640 MB at 1.7 TB/s; one of 61 nodes, 64 / 8 heads, over 16381 keys: 144 us, 229
+// TFLOP/s; one of 8 nodes over 509 keys: 14.1 us, latency.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -160,7 +161,7 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ float ktu_exp2(float x) {       // 2^x, x <= 15; -inf gives 0
+__device__ __forceinline__ float ktu_exp2(float x) {       // 2^x to about 2^-22 of it, x <= 15; -inf gives 0
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;

@@ -272,7 +272,8 @@ class KVCache:
 
         Node i attends the keys [0, lens[b]) and slot lens[b] + j for every bit j of mask[b,i] (int64 [B,T], or [T] for one tree
         for all: see tree_mask); a node that attends nothing gives 0.  Lk: keys that any sequence can attend, the nodes included;
-        lens int32 [B], default Lk - T."""
+        lens int32 [B], default Lk - T.  Head dimension 128, gs = 2 and a capacity that is a multiple of 16 run on the tuned kernel,
+        other caches 9 to 40 times slower."""
         if int(q.shape[0]) != self.B:
             raise ValueError("q has %d sequences, the cache %d" % (int(q.shape[0]), self.B))
         return _OPS.kv_tree_attention(q, *self.k, *self.v, mask, lens, self.Hkv, int(Lk), self.D, self.nb, self.u, self.gs, self.Lcap,
