@@ -15,6 +15,10 @@ D = 128
 RAGGED = [5900, 130, 260, 2000, 5, 383, 6000, 1400, 77, 3100]
 
 
+def _gen(rng):
+    return torch.Generator(device="cuda").manual_seed(int(rng.integers(1 << 30)))
+
+
 def _fields(plane, width, count):
     """Bytes [..., n] of a dense little-endian run of two's-complement fields -> float64 [..., count]."""
     bits = (plane[..., None] >> torch.arange(8, device="cuda", dtype=torch.uint8)) & 1
@@ -78,7 +82,7 @@ def _case(rng, B, T, Hq, Hkv, u, lens, edit=None, aim=0.0, scale=1.0, least=4.0)
     assert _tiles(lens, T, Hkv, Hq // Hkv) >= least * sms
     Lk = int(max(lens)) + T
     c = _cache(B, Hkv, D, (Lk + 15) // 16 * 16, u, 2, fill=0x7F)
-    g = torch.Generator(device="cuda").manual_seed(int(rng.integers(1 << 30)))
+    g = _gen(rng)
     w = torch.randn((1, Hkv, 1, D), generator=g, device="cuda")
     K, V = (torch.randn((B, Hkv, Lk, D), generator=g, device="cuda") for _ in range(2))
     K += aim * w * (torch.arange(Lk, device="cuda") / Lk)[:, None]
@@ -218,10 +222,10 @@ KERNELS = [(4, 2, 0), (3, 2, 0), (2, 2, 0), (4, 8, 0), (4, 2, 1)]
 @pytest.mark.parametrize("ctx", [1, 4096])
 def test_large_values_average_to_finite_numbers(rng, u, gs, odd, bits, ctx):
     """One key of 2^bits, or 4096 of them, and among the nodes one with a weight of 2^-30 and one of 2^-60 in front of them."""
-    T = 4
+    T, g = 4, _gen(rng)
     K, V = torch.zeros((ctx + T, D), device="cuda"), torch.ones((ctx + T, D), device="cuda")
-    V[:ctx] *= 2.0 ** bits * (1 + 0.9 * torch.rand((ctx, D), device="cuda"))
-    V[ctx:] = torch.randn((T, D), device="cuda")
+    V[:ctx] *= 2.0 ** bits * (1 + 0.9 * torch.rand((ctx, D), generator=g, device="cuda"))
+    V[ctx:] = torch.randn((T, D), generator=g, device="cuda").clamp(-3.9, 3.9)          # (times 2^126 still a number)
     V[ctx + 1] *= 2.0 ** bits
     K[ctx + 1, 0], K[ctx + 2, 0] = -235.0, -470.0              # e^(-235 / sqrt(128)) = 2^-30
     seen = [{0}, {0, 1}, {0, 2}, {3}]
@@ -236,10 +240,10 @@ def test_large_values_average_to_finite_numbers(rng, u, gs, odd, bits, ctx):
 def test_small_values_beside_large_ones(rng, u, gs, odd, bits):
     """Nodes that attend only small values keep their digits beside nodes that attend large ones: a large value with a weight of 2^-30
     is a large number, the others are as if it were not there."""
-    T, ctx = 6, 0
-    K, V = torch.zeros((T, D), device="cuda"), torch.randn((T, D), device="cuda")
+    T, ctx, g = 6, 0, _gen(rng)
+    K, V = torch.zeros((T, D), device="cuda"), torch.randn((T, D), generator=g, device="cuda")
     V[1] *= 2.0 ** -60
-    V[3] = 2.0 ** bits * (1 + 0.9 * torch.rand(D, device="cuda"))
+    V[3] = 2.0 ** bits * (1 + 0.9 * torch.rand(D, generator=g, device="cuda"))
     K[3, 0] = -235.0
     seen = [{0}, {1}, {0, 2}, {2, 3}, {4}, {1, 5}]
     got, ref, mag, big, all_v = _nodes_only(rng, u, gs, 16 + odd, T, ctx, K, V, seen)
@@ -264,7 +268,7 @@ def test_values_without_a_finite_number(rng, u):
     """An infinity: NaN in the rows that attend it, the others as without it.  The largest finite values are numbers."""
     T, ctx = 5, 3
     for value in (2.0 ** 127, np.inf, -np.inf):
-        K, V = torch.zeros((ctx + T, D), device="cuda"), torch.randn((ctx + T, D), device="cuda")
+        K, V = torch.zeros((ctx + T, D), device="cuda"), torch.randn((ctx + T, D), generator=_gen(rng), device="cuda")
         V[ctx + 2, 77] = value
         seen = [{0}, {1}, {0, 2}, {2}, {0, 4}]
         c = _cache(1, 1, D, 16, u, 2, rotate=False)
@@ -289,7 +293,7 @@ def test_values_without_a_finite_number(rng, u):
 def test_values_next_to_the_smallest_that_the_format_holds(rng, bits):
     """The quantiser's smallest block (2^-100 and below) counts as zeros; what is larger counts."""
     T, ctx = 2, 130
-    K, V = torch.zeros((ctx + T, D), device="cuda"), 2.0 ** bits * (1 + 0.9 * torch.rand((ctx + T, D), device="cuda"))
+    K, V = torch.zeros((ctx + T, D), device="cuda"), 2.0 ** bits * (1 + 0.9 * torch.rand((ctx + T, D), generator=_gen(rng), device="cuda"))
     got, ref, mag, big, all_v = _nodes_only(rng, 4, 2, 144, T, ctx, K, V, [{0}, {0, 1}])
     lim = _bound(ref, mag, big, all_v, 2.0 ** -15) - 1e-30
     assert (np.abs(got - ref) <= lim).all()
