@@ -12,13 +12,12 @@ struct TreePlan {
     int S, key_tile, groups, rows;
 };
 
-// Rows per thread block by the rows there are: blocks of 16 / 32 / 64 took, us, over 4 sequences of 32752 keys and 8 kv heads: 16 rows 93 /
-// 114 / 119, 32 rows 172 / 115 / 120, 64 rows 331 / 214 / 124; 16 sequences of 2000: 38 / 48 / 59, 63 / 52 / 63, 110 / 89 / 66; one of
-// 16000: 16 rows 28 / 34 / 40, 32 rows 38 / 35 / 42.  Fewer where every block still has one tile at most: the keys are decoded more often, by
-// SMs that had nothing to do (one sequence, 8 kv heads: 32 rows over 509 keys 16.1 -> 13.4, 64 rows over 100 keys 19.6 -> 12.1, over
-// 509 20.6 -> 16.3; up to two tiles: 488 rows over 100 keys 23.6 -> 26.9, no) -- not under the hook that stops the first block's
-// products, which then stops all rows of a small item.  As many runs of the line of tiles as there are SMs, or
-// as there can be tiles.
+// Rows per thread block by the rows there are: blocks of 16 / 32 / 64 took, us, over 4 sequences of 32752 keys and 8 kv heads: 16 rows 85 /
+// 93 / 118, 32 rows 157 / 93 / 120, 64 rows 300 / 170 / 123; 16 sequences of 2000: 35 / 41 / 59, 57 / 43 / 64, 100 / 71 / 66; one of
+// 16000: 16 rows 27 / 30 / 41, 32 rows 35 / 31 / 42.  Fewer where every block still has one tile at most: the keys are decoded more often, by
+// SMs that had nothing to do (one sequence, 8 kv heads: 32 rows over 509 keys 14.1 -> 12.5, 64 rows over 100 keys 19.6 -> 11.1, over
+// 509 20.5 -> 14.2; up to two tiles: 488 rows over 16 keys 14.8 -> 17.7, no) -- not under the hook that stops the first block's
+// products, which then stops all rows of a small item.  As many runs of the line of tiles as there are SMs, or as there can be tiles.
 TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
     TreePlan p;
     const int64_t R = T * (H / Hkv);
@@ -32,7 +31,7 @@ TreePlan plan_tree_umma(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk
 }
 
 // The tuned kernel: head_dim 128, gs = 2, capacity a multiple of 16 (and planes on 16-byte boundaries: bulk copies), tiles counted in 31 bits.
-// (The generic kernel takes 121 instead of 13.3 us at 8 nodes over 509 keys, 16.2 ms instead of 0.41 for 16 sequences of 16 nodes over up to
+// (The generic kernel takes 121 instead of 12.5 us at 8 nodes over 509 keys, 16.2 ms instead of 0.41 for 16 sequences of 16 nodes over up to
 // 32752 keys.)
 bool umma_eligible(int64_t D, int gs, int64_t Lcap, int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk) {
     return D == 128 && gs == 2 && Lcap % 16 == 0 && B * Hkv * plan_tree_umma(B, T, H, Hkv, Lk).groups <= INT32_MAX / ((Lk + KTU_KEYS - 1) / KTU_KEYS);
@@ -48,7 +47,7 @@ int launch_tree_umma_rows(const KvTreeArgs& a, const TreePlan& p, int B, __nv_bf
             return fail(MSAQ_ERR_CUDA, "cannot reserve %d bytes of shared memory", smem);
         configured[dev] = true;
     }
-    launch_chained(kv_tree_umma_kernel<U, NR>, dim3((unsigned)p.S), dim3(ktu_threads(NR)), smem, st, a, B, p.groups, out, out_f32);
+    launch_chained(kv_tree_umma_kernel<U, NR>, dim3((unsigned)p.S), dim3(KTU_THREADS), smem, st, a, B, p.groups, out, out_f32);
     count_launch();
     if (int rc = check_launch("kv_tree_umma")) return rc;
     launch_chained(kv_tree_merge_kernel<NR>, dim3((unsigned)(a.Hkv * p.groups * (NR / 8)), (unsigned)B), dim3(256), 0, st, a, B, p.groups, p.S, out,

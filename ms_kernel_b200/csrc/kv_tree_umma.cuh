@@ -21,10 +21,12 @@
 //   * Queries are staged once per item, rotated in fp32, scaled by a power of two and held as two fp16 numbers, the leading eleven digits and
 //     what they leave: 22 digits.  So are probabilities (two bf16 numbers beside values in bf16), 2^7 above the reference's scale so that
 //     they reach down to 2^-31.  With one number each the result before its rounding was off by 1.2e-4 (beside values in bf16 by 1.1e-3);
-//     now by less than 2e-5 (over 32752 keys by 2.5e-5, 1.5e-6 of the average |v|), for 12 % more time (16 sequences of 16 nodes,
-//     below), 9 % (61 nodes), 2 % (8 nodes over 509 keys).  The second numbers of the probabilities are further columns of the same
-//     products: the values are read once.
-//   * Eight softmax warps, thread = (key, half of the rows), four up to 32 rows.  The maximum is lazy: a row's reference moves only when a score
+//     now by less than 2e-5 (over 32752 keys by 2.5e-5, 1.5e-6 of the average |v|), for 9 to 13 % more time with 64 rows, 5 % and less
+//     with fewer.  The second numbers of the probabilities are further columns of the same products: the values are read once.  So are
+//     those of up to 32 queries (4 sequences of 32752 keys, 16 rows 93 -> 83 us, 32 rows 102 -> 93: with few rows a product's time hardly
+//     depends on them); with 64 the softmax pays as much for adding the two shares as the products gain (123 -> 124 us).
+//   * Eight softmax warps, thread = (key, half of the rows) (four up to 16 rows: 16 sequences of 2000 keys 35.8 instead of 34.5 us, 8 nodes over
+//     509 keys 13.4 instead of 12.5, but 4 sequences of 32752 83 instead of 85).  The maximum is lazy: a row's reference moves only when a score
 //     exceeds it by more than 2^8 -- one vote per tile of the four warps that hold the row -- and then the accumulators of the
 //     rows concerned are rescaled in tensor memory.  Sums and accumulators are fp32.
 //   * One warp issues the MMAs: S(i + 1) before P.V(i), so that both run under the decoding and the softmax.
@@ -33,8 +35,8 @@
 //     kernel in the order of the runs.
 // What bounds it: the instructions of decoding and softmax, 7900 of a warp per tile of 128 keys and 64 rows (61 % of the issue
 // slots), and the hand-overs between roles; the tensor cores are busy one cycle in four, HBM one in five.  16 sequences of 16 nodes,
-// 32 / 8 heads, over up to 32752 keys (u = 4): 373 us, 640 MB at 1.7 TB/s; one of 61 nodes, 64 / 8 heads, over 16381 keys: 144 us, 229
-// TFLOP/s; one of 8 nodes over 509 keys: 14.1 us, latency.
+// 32 / 8 heads, over up to 32752 keys (u = 4): 373 to 389 us by the draw, 640 MB at 1.7 TB/s; one of 61 nodes, 64 / 8 heads, over 16381 keys: 144 us, 229
+// TFLOP/s; one of 8 nodes over 509 keys: 13.3 us, latency.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -45,9 +47,8 @@
 namespace msaq {
 
 constexpr int KTU_DEC_WARPS = 16, KTU_KEYS = 128, KTU_ROWS = 64;
-// Softmax warps: two halves of the rows by four quarters of the keys; up to 32 rows one set of four (a warp's work is mostly its waits then).
-__host__ __device__ constexpr int ktu_soft_warps(int nr) { return nr > 32 ? 8 : 4; }
-__host__ __device__ constexpr int ktu_threads(int nr) { return (KTU_DEC_WARPS + ktu_soft_warps(nr) + 4) * 32; }       // and four single ones
+constexpr int KTU_SOFT_WARPS = 8;                                                   // two halves of the rows by four quarters of the keys
+constexpr int KTU_THREADS = (KTU_DEC_WARPS + KTU_SOFT_WARPS + 4) * 32;              // and four single ones
 constexpr int KTU_COL_O = 0, KTU_COL_S = 128, KTU_COL_K = 256, KTU_COLS = 512;      // tensor memory columns: two O, two S, two K (384 used)
 // Shared memory: two buffers of values, probabilities, queries, ring.  Probabilities and queries are stored as two numbers each, the
 // leading digits and what they leave.  Probabilities of up to 32 rows: two buffers, the second numbers of a key right behind the
@@ -58,6 +59,11 @@ __host__ __device__ constexpr int ktu_p_second(int nr) { return nr > 32 ? 16384 
 constexpr int KTU_PART = 132;                                                       // floats of a row's partial result: acc, m, l, padding
 __host__ __device__ constexpr int ktu_ub(int u) { return 4 * (8 - u); }              // bytes of a block: upper codes, shared codes (and an exponent)
 __host__ __device__ constexpr int ktu_sb(int u) { return 2 * u; }
+// Queries, K-major in two halves of 64 channels: up to 32 rows a row's second numbers are further rows of the same product, 64 rows: of
+// one that follows.  Distances between the halves and between the numbers:
+__host__ __device__ constexpr bool ktu_q_joint(int nr) { return nr <= 32; }
+__host__ __device__ constexpr int ktu_q_half(int nr) { return ktu_q_joint(nr) ? nr * 256 : nr * 128; }
+__host__ __device__ constexpr int ktu_q_second(int nr) { return ktu_q_joint(nr) ? nr * 128 : nr * 256; }
 __host__ __device__ constexpr int ktu_stages(int u, int nr) { return u == 4 && nr <= 32 ? 4 : 3; }
 __host__ __device__ constexpr int ktu_stage_bytes(int u) { return 2 * 4 * KTU_KEYS * (ktu_ub(u) + ktu_sb(u) + 1); }
 __host__ __device__ constexpr int ktu_smem_bytes(int u, int nr) { return KTU_Q + nr * 512 + ktu_stages(u, nr) * ktu_stage_bytes(u) + 1024; }
@@ -114,8 +120,9 @@ __device__ __forceinline__ void ktu_st8(uint32_t taddr, const float* v) {
                  "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
                  : "memory");
 }
-// N accumulator columns (16 or 32) in one access.
+// N accumulator columns (8, 16 or 32) in one access.
 template <int N> __device__ __forceinline__ void ktu_ld(uint32_t taddr, float (&v)[N]);
+template <> __device__ __forceinline__ void ktu_ld<8>(uint32_t taddr, float (&v)[8]) { ktu_ld8(taddr, v); }
 template <> __device__ __forceinline__ void ktu_ld<16>(uint32_t taddr, float (&v)[16]) { tmem_ld16(taddr, v); }
 template <> __device__ __forceinline__ void ktu_ld<32>(uint32_t taddr, float (&v)[32]) {
     uint32_t r[32];
@@ -362,11 +369,11 @@ struct __align__(16) KtuShared {
 };
 
 template <int U, int NR>
-__global__ void __launch_bounds__(ktu_threads(NR), 1)
+__global__ void __launch_bounds__(KTU_THREADS, 1)
 kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __restrict__ out, float* __restrict__ out_f32) {
     chain_wait();
     constexpr int PB = ktu_p_buffers(NR);
-    constexpr int SW = ktu_soft_warps(NR), NC = NR / (SW / 4);    // softmax warps; columns (query rows) of a thread in the softmax
+    constexpr int SW = KTU_SOFT_WARPS, NC = NR / 2;               // columns (query rows) of a thread in the softmax
     constexpr int WARP_MMA = KTU_DEC_WARPS + SW, WARP_COPY = WARP_MMA + 1, WARP_SCOUT = WARP_MMA + 2, WARPS = WARP_MMA + 4;
     extern __shared__ uint8_t ktu_smem_raw[];
     __shared__ KtuShared sh;
@@ -470,8 +477,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
 
     if (warp < KTU_DEC_WARPS) {
         // ================================ decode ================================
-        if (SW == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int team = warp >> 3;
         const uint32_t tab = smem_u32(sh.scales);
         int seg = -1;
@@ -530,9 +536,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                         const int p = ktu_place<U>(lane * 4 + i);
                         const float x = bad >> k & 1 ? 0.0f : v[k][i] * up;
                         const __half h = __float2half_rn(x);
-                        __half* const to = reinterpret_cast<__half*>(smem + KTU_Q + (p >> 6) * (NR * 128) + r * 128 + ((((p >> 3) & 7) ^ (r & 7)) << 4) + (p & 7) * 2);
+                        __half* const to = reinterpret_cast<__half*>(smem + KTU_Q + (p >> 6) * ktu_q_half(NR) + r * 128 + ((((p >> 3) & 7) ^ (r & 7)) << 4) + (p & 7) * 2);
                         to[0] = h;
-                        to[NR * 128] = __float2half_rn(x - __half2float(h));
+                        to[ktu_q_second(NR) / 2] = __float2half_rn(x - __half2float(h));
                     }
                     if (lane == 0) sh.qf[seg & 3][r] = bad >> k & 1 ? __int_as_float(0x7FC00000) : exp2_int(e - 10);
                 }
@@ -609,8 +615,7 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
         }
     } else if (warp < WARP_MMA) {
         // ================================ softmax ================================
-        if (SW == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
         const uint32_t prow = (sbase + KTU_P + (key >> 3) * 1024 + (key & 7) * 128) | (key & 7) << 4;
         const int stid = tid - KTU_DEC_WARPS * 32, htid = stid & 127;             // thread of the role, of its half
         int seg = -1, n_seg = 0;
@@ -663,6 +668,12 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             float x[NC];
             auto scores = [&]() {                                 // exponents of this tile's probabilities on the present references
                 ktu_ld<NC>(scol, x);
+                if constexpr (ktu_q_joint(NR)) {                  // the second numbers' share
+                    float x2[NC];
+                    ktu_ld<NC>(scol + NR, x2);
+#pragma unroll
+                    for (int c = 0; c < NC; c += 2) unpack2(add2(pack2(x[c], x[c + 1]), pack2(x2[c], x2[c + 1])), x[c], x[c + 1]);
+                }
                 const uint64_t ck2 = pack2(ck, ck);
                 if (!same)
 #pragma unroll
@@ -700,6 +711,12 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
                 for (int c = 0; c < NC; c += 8) {
                     float s[8];
                     ktu_ld8(scol + c, s);
+                    if constexpr (ktu_q_joint(NR)) {
+                        float s2[8];
+                        ktu_ld8(scol + NR + c, s2);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) s[k] += s2[k];
+                    }
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int r = half * NC + c + k;
@@ -835,12 +852,11 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             cur.next(a, groups, B);
         }
     } else {
-        if (SW == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     }
     if (warp == WARP_MMA) {
         // ================================ MMAs ================================
-        const uint32_t idesc_qk = ktu_idesc(NR, 0, 0), hi = ktu_desc_hi(1024);
+        const uint32_t idesc_qk = ktu_idesc(ktu_q_joint(NR) ? 2 * NR : NR, 0, 0), hi = ktu_desc_hi(1024);
         const uint32_t q_lo = umma_desc_lo(sbase + KTU_Q, 16), v_lo = umma_desc_lo(sbase + KTU_V, 16384), p_lo = umma_desc_lo(sbase + KTU_P, 16384);
         int seg = -1;
         KtuCursor ahead = cur;                                    // of the scores' product, one tile in front
@@ -854,9 +870,9 @@ kv_tree_umma_kernel(const KvTreeArgs a, int B, int groups, __nv_bfloat16* __rest
             tc_fence_after();
             if (elect_lane()) {
 #pragma unroll 1
-                for (int s = 0; s < 16; ++s)                      // keys by the queries' first numbers, by their second ones
+                for (int s = 0; s < (ktu_q_joint(NR) ? 8 : 16); ++s)     // keys by the queries' first numbers and their second ones
                     ktu_mma_ts(tm + KTU_COL_S + (j & 1) * 64, tm + KTU_COL_K + (j & 1) * 64 + 8 * (s & 7),
-                               q_lo + (s >> 2) * (NR * 8) + (s & 3) * 2, hi, idesc_qk, s > 0);
+                               q_lo + (s >> 2) * (ktu_q_half(NR) / 16) + (s & 3) * 2, hi, idesc_qk, s > 0);
                 if (!(a.skip_stage == j && blockIdx.x == 0)) tc_commit(smem_u32(&sh.sfull[j & 1]));
             }
             __syncwarp();

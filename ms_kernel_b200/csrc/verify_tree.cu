@@ -17,7 +17,7 @@
 // element's value after n rejections follows from p, q and the n factors Z.  The code is kept small: unrolled further, with a loop
 // over the rejections around each element, the kernel spent most of its time fetching instructions (one sequence, 8 nodes, 32000
 // entries, no draft: 27 us, now 8.0 of which 5.2 on the device; 16 sequences, 64 nodes, 128256 entries, up to five
-// rejections in a row: 75 us, now 35 to 53 by the draw).
+// rejections in a row: 75 us, now 35 to 61 by the draw).
 #include "msaq_common.cuh"
 #include "sm100_ptx.cuh"
 
