@@ -387,7 +387,7 @@ int msaq_kv_write_qkv(const void* qkv, int64_t ld, void* q_out, int8_t* k_scale_
  * they hold.  lens int32 [B], clipped to [0, Lk - T]; NULL: Lk - T for every sequence.  Lk: keys that any sequence can attend, the
  * nodes included, 2^30 at most (it sets the split of the keys).  qrot as for msaq_kv_decode_attention_batched.  Any H / Hkv; formats and head
  * dimensions as for the decode.  out_f32 (optional) also receives the result before its rounding.  An average of finite values is finite
- * whatever their size; a row that attends an infinite value (a value block of exponent 122 or more) is not finite, in its channel at
+ * whatever their size, and values below 2^-99, the quantiser's smallest, may count as 0; a row that attends an infinite value (a value block of exponent 122 or more) is not finite, in its channel at
  * least.  workspace: on a 16-byte boundary.
  */
 size_t msaq_kv_tree_workspace(int64_t B, int64_t T, int64_t H, int64_t Hkv, int64_t Lk, int64_t D);
